@@ -1,4 +1,4 @@
-"""ctypes bindings of the four kernel libraries (the reference's own FFI style, e.g. rmsnorm/candidate.py:25-28).
+"""ctypes bindings of the kernel libraries (the reference's own FFI style, e.g. rmsnorm/candidate.py:25-28).
 
 A library that is missing raises at first use: there is no CPU or PyTorch fallback for any op. Every binding takes
 plain pointers, sizes and the caller's CUDA stream, exactly as declared in include/ckb200_<op>.h.
@@ -29,6 +29,7 @@ SIGNATURES = {
         "launch": (_INT, [_VP] * 7 + [_LL] + [_INT] * 7 + [_VP]),
         "ckb_rope_sincos_launch": (_INT, [_VP] * 6 + [_LL] + [_INT] * 4 + [_VP]),
         "ckb_rope_kv_cache_launch": (_INT, [_VP] * 11 + [_LL] + [_INT] * 5 + [_VP]),
+        "ckb_rope_qk_norm_launch": (_INT, [_VP] * 15 + [_LL] * 4 + [_INT] * 6 + [_FLT, _VP]),
     },
     "topk": {
         "plan": (_LL, [_LL, _LL, _INT, _INT, _INT, _INT]),
@@ -46,6 +47,9 @@ SIGNATURES = {
         "ckb_p2p_import": (_INT, [_VP, _PVP]),
         "ckb_p2p_close": (_INT, [_VP]),
         "ckb_topk_status": (_INT, [_INT]),
+    },
+    "verify": {
+        "ckb_verify_launch": (_INT, [_VP] * 7 + [_LL] * 5 + [_INT] * 3 + [_VP]),
     },
 }
 

@@ -3,14 +3,17 @@
 The reference's rope/candidate.py:44-57: q [B, S, Hq, D] and k [B, S, Hkv, D] in bf16 or fp16 are rotated by the
 cos/sin cache rows [max_position, D] (fp32, bf16 or fp16) that position_ids [B, S] (int64) pick, half-split pairing,
 fp32 math with each product and the sum rounded, one rounding to the output dtype (rope/kernel.cu:1-8).
-Extensions, both through this module's inputs:
+Extensions through this module's inputs:
   * inputs["inplace"] = True rotates q and k in place (they must be contiguous) and returns them as q_out / k_out;
   * no "cos"/"sin" but inputs["theta"] computes cos/sin in registers by sincosf(position * inv_freq) with
     inv_freq = 1 / theta^(2i / D) (the cat(freqs, freqs) cache layout), so no cache is read.
+rope_kv_cache writes the rotated keys and the values into a paged cache on the way; qk_norm_rope and
+qk_norm_rope_kv_cache norm each query and key head first (a model with query and key norms), in the same pass.
 params.json beside this module may set "rows" and "splits" as the reference's does; they are validated by the C ABI
 and do not change the B200 launch shape.
 """
 
+import ctypes
 import json
 import os
 
@@ -149,3 +152,116 @@ def rope_kv_cache(q, k, v, position_ids, cos, sin, key_cache, value_cache, slot_
                                            _QK[q.dtype], _CACHE[cos.dtype], _native.stream_of(q))
     _native.check(err)
     return q_out, k_out
+
+
+_STRIDES = ctypes.c_longlong * 15
+
+
+def _strides(t):
+    """The batch, token and head strides of a [B, S, heads, D] view (0 for a dim of size 1, whose stride is any)."""
+    return [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()[:3])]
+
+
+def _strided(t, name=None):
+    """t where its last dim is contiguous (a view of a fused projection is), else a contiguous copy; with a name (of an
+    in-place output) a tensor that cannot be written through its view raises."""
+    unit = t.shape[3] == 1 or t.stride(3) == 1
+    if name is None:
+        return t if unit else t.contiguous()
+    if not unit or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"rope candidate: in-place rotation needs {name} with a contiguous last dim and no expanded dim")
+    return t
+
+
+def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches, slot_mapping, eps, inplace, write_k, out):
+    if (cos is None) != (sin is None) or (cos is None) == (theta is None):
+        raise ValueError("rope candidate: give the cos/sin cache (both) or theta")
+    problem = _problem(q, k, cos, sin, position_ids)
+    if problem:
+        raise ValueError(f"rope candidate: {problem}")
+    q_heads, kv_heads, head_dim = q.shape[2], k.shape[2], q.shape[3]
+    if q_heads < 1 or kv_heads < 1 or head_dim < 2:
+        raise ValueError(f"rope candidate: shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype not in _CACHE or w.dtype != q_weight.dtype or tuple(w.shape) != (head_dim,):
+            raise ValueError(f"rope candidate: {name} must be [{head_dim}] of fp32, bf16 or fp16 (both the same), got "
+                             f"{w.dtype} {tuple(w.shape)}")
+    if cos is not None and cos.shape[0] < 1:
+        raise ValueError("rope candidate: the cos/sin cache has no rows")
+    tensors = [q, k, position_ids, q_weight, k_weight] + ([] if cos is None else [cos, sin])
+    slots = None
+    if caches is not None:
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"rope candidate: v {v.dtype} {tuple(v.shape)} must match k {k.dtype} {tuple(k.shape)}")
+        for name, c in zip(("key_cache", "value_cache"), caches):
+            if c.dtype != q.dtype or c.dim() != 4 or tuple(c.shape[2:]) != tuple(k.shape[2:]) or not c.is_contiguous():
+                raise ValueError(f"rope candidate: {name} must be a contiguous [blocks, block_size, {kv_heads}, "
+                                 f"{head_dim}] tensor of {q.dtype}, got {c.dtype} {tuple(c.shape)}")
+        if caches[0].shape != caches[1].shape:
+            raise ValueError(f"rope candidate: key_cache {tuple(caches[0].shape)} and value_cache "
+                             f"{tuple(caches[1].shape)} differ")
+        if slot_mapping.dtype != torch.int64 or tuple(slot_mapping.shape) != tuple(position_ids.shape):
+            raise ValueError(f"rope candidate: slot_mapping must be int64 {tuple(position_ids.shape)}")
+        tensors += [v, *caches, slot_mapping]
+    _native.require_cuda("rope", *tensors)
+    if inplace:
+        q_out, k_out = _strided(q, "q"), (_strided(k, "k") if write_k else None)
+        q, k = q_out, k if k_out is not None else _strided(k)
+    else:
+        q, k = _strided(q), _strided(k)
+        if out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if write_k else None
+        else:
+            q_out, k_out = out
+            for o, t in ((q_out, q), (k_out, k)):
+                if o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous() or o.device != t.device:
+                    raise ValueError("rope candidate: out must be contiguous tensors of q's and k's shapes, dtype "
+                                     "and device")
+    if caches is not None:
+        v, slots = _strided(v), slot_mapping.contiguous()
+    ids, q_weight, k_weight = position_ids.contiguous(), q_weight.contiguous(), k_weight.contiguous()
+    strides = _STRIDES(*_strides(q), *_strides(k), *(_strides(v) if caches is not None else (0, 0, 0)), *_strides(q_out),
+                       *(_strides(k_out) if k_out is not None else (0, 0, 0)))
+    batch, seq = ids.shape
+    lib = _native.load("rope")
+    with torch.cuda.device(q.device):
+        freqs = None
+        if cos is None:
+            freqs = inv_freq(theta, head_dim, q.device)
+        else:
+            cos, sin = cos.contiguous(), sin.contiguous()
+
+        def ptr(t):
+            return None if t is None else t.data_ptr()
+
+        key_cache, value_cache = caches if caches is not None else (None, None)
+        err = lib.ckb_rope_qk_norm_launch(ptr(q), ptr(k), ptr(v if caches is not None else None), ptr(q_weight),
+                                          ptr(k_weight), ptr(cos), ptr(sin), ptr(freqs), ptr(ids), ptr(slots),
+                                          ptr(q_out), ptr(k_out), ptr(key_cache), ptr(value_cache), strides,
+                                          0 if cos is None else cos.shape[0],
+                                          0 if key_cache is None else key_cache.shape[0] * key_cache.shape[1], batch,
+                                          seq, q_heads, kv_heads, head_dim, _QK[q.dtype], _CACHE[q_weight.dtype],
+                                          0 if cos is None else _CACHE[cos.dtype], float(eps), _native.stream_of(q))
+    _native.check(err)
+    return q_out, k_out
+
+
+def qk_norm_rope(q, k, position_ids, q_weight, k_weight, cos=None, sin=None, theta=None, eps=1e-6, inplace=False,
+                 out=None):
+    """RMSNorm of every query and key head over head_dim, then the rotation, in one kernel: each head x of q
+    [B, S, Hq, D] becomes rotate(x * rsqrt(mean(x^2) + eps) * q_weight) and each head of k [B, S, Hkv, D] the same with
+    k_weight ([D], fp32, bf16 or fp16), fp32 math with one rounding at the end. q and k may be views of a fused
+    projection (any strides, the last dim contiguous). cos / sin [max_position, D] picked by position_ids (an id
+    outside takes the nearest row), or theta; inplace and out as in rope(). Returns (q_out, k_out)."""
+    return _qk_norm(q, k, None, position_ids, q_weight, k_weight, cos, sin, theta, None, None, eps, inplace, True, out)
+
+
+def qk_norm_rope_kv_cache(q, k, v, position_ids, q_weight, k_weight, cos, sin, key_cache, value_cache, slot_mapping,
+                          theta=None, eps=1e-6, inplace=True, write_k=True):
+    """qk_norm_rope fused with the paged KV-cache write, one kernel: the normed and rotated k and the v [B, S, Hkv, D]
+    as it is of token (b, s) are stored at slot slot_mapping[b, s] of key_cache / value_cache [num_blocks, block_size,
+    Hkv, D], as rope_kv_cache does (a slot outside the caches, a padding token's, is not written). q, k and v may be
+    views of a fused projection; in place writes through them. Returns (q_out, k_out or None)."""
+    return _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, (key_cache, value_cache), slot_mapping,
+                    eps, inplace, write_k, None)

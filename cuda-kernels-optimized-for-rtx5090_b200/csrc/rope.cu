@@ -429,6 +429,8 @@ bool bad_shape(long long tokens, int q_heads, int kv_heads, int head_dim) {
 }  // namespace
 }  // namespace ckb
 
+#include "rope_qk_norm.cuh"
+
 using namespace ckb;
 
 // Replaces the reference's rope `launch` (rope/kernel.cu:201-215): same arguments, checks and return codes. `rows` and
@@ -480,5 +482,36 @@ CKB_EXPORT int ckb_rope_kv_cache_launch(const void* q, const void* k, const void
                  key_cache, value_cache, tokens, q_heads, kv_heads, head_dim};
   if (qk_dtype == kBF16) return start_kv_cache<__nv_bfloat16>(cache_dtype, a, stream);
   if (qk_dtype == kF16) return start_kv_cache<__half>(cache_dtype, a, stream);
+  return -1;
+}
+
+// RMSNorm of each query and key head, rotated in the same pass (rope_qk_norm.cuh). strides: 15 host values, the batch,
+// token and head strides in elements of q, k, v, q_out and k_out ([batch, seq, heads, head_dim] views with a contiguous
+// last dim). cos_rows null takes inv_freq instead (as ckb_rope_sincos_launch). slots null: no cache write, and v, its
+// strides and the caches are not looked at; k_out null: the keys go to the cache only.
+CKB_EXPORT int ckb_rope_qk_norm_launch(const void* q, const void* k, const void* v, const void* q_weight,
+                                       const void* k_weight, const void* cos_rows, const void* sin_rows,
+                                       const float* inv_freq, const void* ids, const void* slots, void* q_out,
+                                       void* k_out, void* key_cache, void* value_cache, const long long* strides,
+                                       long long positions, long long cache_slots, long long batch, long long seq,
+                                       int q_heads, int kv_heads, int head_dim, int qk_dtype, int w_dtype,
+                                       int cache_dtype, float eps, cudaStream_t stream) {
+  if (batch <= 0 || seq <= 0) return 0;
+  if (batch > INT_MAX || seq > INT_MAX || bad_shape(batch * seq, q_heads, kv_heads, head_dim) ||
+      (long long)q_heads + 2LL * kv_heads > INT_MAX / 8 || strides == nullptr || q == nullptr || k == nullptr ||
+      q_weight == nullptr || k_weight == nullptr || ids == nullptr || q_out == nullptr || w_dtype < kF32 ||
+      w_dtype > kF16 || cache_dtype < kF32 || cache_dtype > kF16)
+    return -1;
+  if (cos_rows == nullptr ? inv_freq == nullptr : sin_rows == nullptr || positions <= 0) return -1;
+  if (slots == nullptr ? k_out == nullptr : v == nullptr || key_cache == nullptr || value_cache == nullptr) return -1;
+  const auto view = [strides](int i) { return View{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
+  const NormArgs a{q, k, v, q_weight, k_weight, cos_rows, sin_rows, inv_freq, (const long long*)ids,
+                   (const long long*)slots, q_out, k_out, key_cache, value_cache, view(0), view(1), view(2), view(3),
+                   view(4), positions, cache_slots, (unsigned)(batch * seq), (unsigned)seq, q_heads, kv_heads, head_dim, w_dtype, cache_dtype,
+                   eps};
+  const bool cache = cos_rows != nullptr;
+  if (qk_dtype == kBF16)
+    return cache ? start_qk_norm<__nv_bfloat16, true>(a, stream) : start_qk_norm<__nv_bfloat16, false>(a, stream);
+  if (qk_dtype == kF16) return cache ? start_qk_norm<__half, true>(a, stream) : start_qk_norm<__half, false>(a, stream);
   return -1;
 }

@@ -35,6 +35,22 @@ int ckb_rope_kv_cache_launch(const void* q, const void* k, const void* v, const 
                              void* value_cache, long long tokens, int q_heads, int kv_heads, int head_dim,
                              int qk_dtype, int cache_dtype, cudaStream_t stream);
 
+/* RMSNorm of each query and key head over head_dim, then launch()'s rotation, in one pass: y = x * rsqrt(mean(x^2) +
+ * eps) * weight, rotated, fp32 throughout with one rounding to qk_dtype. q, k, v, q_out, k_out are [batch, seq, heads,
+ * head_dim] views with a contiguous last dim; strides (host memory) holds the batch, token and head strides of each, in
+ * that order, in elements (15 values). q_weight / k_weight [head_dim] of w_dtype 0 (fp32), 1 (bf16) or 2 (fp16). cos_rows
+ * / sin_rows as launch()'s (cache_dtype), or both null and inv_freq as ckb_rope_sincos_launch's. slots, v, key_cache and
+ * value_cache as ckb_rope_kv_cache_launch's, or slots null: no cache write. positions: rows of cos_rows (a position
+ * outside is taken as the nearest); cache_slots: rows of the caches (a slot outside is not written). q_out == q, k_out == k with their strides
+ * works in place; k_out null (with slots only) leaves k as it is. batch * seq <= INT_MAX. No counterpart in the
+ * reference, whose RMSNorm has no weight and whose RoPE no norm (rmsnorm/kernel.cu:1, rope/kernel.cu:1-13). */
+int ckb_rope_qk_norm_launch(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                            const void* cos_rows, const void* sin_rows, const float* inv_freq, const void* ids,
+                            const void* slots, void* q_out, void* k_out, void* key_cache, void* value_cache,
+                            const long long* strides, long long positions, long long cache_slots, long long batch,
+                            long long seq, int q_heads, int kv_heads, int head_dim, int qk_dtype, int w_dtype,
+                            int cache_dtype, float eps, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
