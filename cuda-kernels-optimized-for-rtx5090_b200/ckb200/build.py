@@ -1,4 +1,5 @@
-"""In-tree build of the four kernel libraries for sm_100a.
+"""In-tree build of the kernel libraries for sm_100a: one for each op of the reference (OPS) and for each op that
+stands beside them (SERVING_OPS).
 
 Each op compiles from csrc/<op>.cu into lib/<op>/libkernel.so, the layout the reference's Python wrappers load
 (`$CKOPT_BUILD_DIR/libkernel.so`, e.g. rmsnorm/candidate.py:25): pointing CKOPT_BUILD_DIR at lib/<op> makes the
@@ -17,6 +18,8 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_ROOT = os.path.join(PKG_ROOT, "lib")
 OPS = ("softmax", "rmsnorm", "rope", "topk")
+SERVING_OPS = ("verify",)  # ops without a counterpart in the reference, under their own symbols
+LIBS = OPS + SERVING_OPS
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -65,7 +68,7 @@ def _compile(op, verbose):
     return out
 
 
-def build(force=False, verbose=False, ops=OPS):
+def build(force=False, verbose=False, ops=LIBS):
     """Compiles every stale (or, with force, every) op library; returns the library paths."""
     todo = [op for op in ops if force or _stale(op)]
     with ThreadPoolExecutor(max_workers=len(todo) or 1) as pool:

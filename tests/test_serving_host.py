@@ -1,0 +1,131 @@
+"""The serving operators on the CPU: what their entry points refuse, in Python and at the C ABI, before any CUDA call; the
+declared symbols; and the oracles' own forms."""
+
+import ctypes
+
+import pytest
+import torch
+
+from ckb200 import _native, build, rope, verify
+from oracle import serving
+from test_abi import declared
+
+
+@pytest.fixture(scope="module", autouse=True)
+def libs():
+    build.build()
+
+
+@pytest.mark.parametrize("op", build.SERVING_OPS)
+def test_library_exports_every_declared_symbol(op):
+    names = declared(op)
+    lib = ctypes.CDLL(build.lib_path(op))
+    assert names and all(hasattr(lib, n) for n in names)
+    assert names == set(_native.SIGNATURES[op])
+
+
+def _qk(**change):
+    a = dict(q=torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), k=torch.zeros(2, 3, 2, 64, dtype=torch.bfloat16),
+             position_ids=torch.zeros(2, 3, dtype=torch.int64), q_weight=torch.ones(64), k_weight=torch.ones(64),
+             cos=torch.zeros(8, 64), sin=torch.zeros(8, 64))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros(2, 3, 4, 64)), dict(k=torch.zeros(2, 3, 2, 64, dtype=torch.float16)),
+    dict(k=torch.zeros(2, 3, 2, 32, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 3, 0, 64, dtype=torch.bfloat16)),
+    dict(q_weight=torch.ones(32)), dict(k_weight=torch.ones(64, dtype=torch.bfloat16)), dict(q_weight=torch.ones(64).double()),
+    dict(cos=None), dict(cos=None, sin=None), dict(theta=1e4), dict(cos=torch.zeros(8, 32), sin=torch.zeros(8, 32)),
+    dict(cos=torch.zeros(0, 64), sin=torch.zeros(0, 64)), dict(position_ids=torch.zeros(2, 3, dtype=torch.int32)),
+    dict(position_ids=torch.zeros(3, 2, dtype=torch.int64)), {}])
+def test_qk_norm_rope_refusals(change):
+    with pytest.raises(ValueError, match="CUDA" if not change else "^rope candidate"):
+        rope.qk_norm_rope(**_qk(**change))
+
+
+def _cached(**change):
+    a = dict(_qk(), v=torch.zeros(2, 3, 2, 64, dtype=torch.bfloat16), slot_mapping=torch.zeros(2, 3, dtype=torch.int64),
+             key_cache=torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16), value_cache=torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(v=torch.zeros(2, 3, 2, 64)), dict(v=torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16)),
+    dict(key_cache=torch.zeros(4, 16, 2, 64)), dict(value_cache=torch.zeros(4, 16, 4, 64, dtype=torch.bfloat16)),
+    dict(value_cache=torch.zeros(5, 16, 2, 64, dtype=torch.bfloat16)),
+    dict(key_cache=torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16).transpose(1, 2)),
+    dict(slot_mapping=torch.zeros(2, 3, dtype=torch.int32)), dict(slot_mapping=torch.zeros(6, dtype=torch.int64)), {}])
+def test_qk_norm_rope_kv_cache_refusals(change):
+    with pytest.raises(ValueError, match="CUDA" if not change else "^rope candidate"):
+        rope.qk_norm_rope_kv_cache(**_cached(**change))
+
+
+def test_in_place_refuses_what_cannot_be_written():
+    with pytest.raises(ValueError, match="expanded"):
+        rope._strided(torch.zeros(1, 1, 1, 64).expand(2, 3, 4, 64), "q")
+    with pytest.raises(ValueError, match="contiguous last dim"):
+        rope._strided(torch.zeros(2, 3, 64, 4).transpose(2, 3), "q")
+    x = torch.zeros(2, 3, 8, 64)[:, :, 2:6]
+    assert rope._strided(x) is x and rope._strided(x, "q") is x
+
+
+def test_qk_norm_abi_refusals():
+    fn = _native.load("rope").ckb_rope_qk_norm_launch
+    p = 16  # a pointer that is only compared with null: every call below returns before a launch
+    strides = (ctypes.c_longlong * 15)()
+    good = [p, p, p, p, p, p, p, None, p, p, p, p, p, p, strides, 8, 64, 2, 3, 4, 2, 64, 1, 0, 0, 1e-6, None]
+
+    def call(**at):
+        a = list(good)
+        for i, v in at.items():
+            a[int(i[1:])] = v
+        return fn(*a)
+
+    assert call(_17=0) == 0 and call(_18=0) == 0  # no tokens
+    for change in (dict(_0=None), dict(_1=None), dict(_2=None), dict(_3=None), dict(_4=None), dict(_6=None), dict(_8=None),
+                   dict(_10=None), dict(_12=None), dict(_13=None), dict(_14=None), dict(_15=0), dict(_17=1 << 31),
+                   dict(_17=1 << 20, _18=1 << 20), dict(_19=0), dict(_20=0), dict(_21=63), dict(_21=0), dict(_22=0),
+                   dict(_22=3), dict(_23=3), dict(_24=-1), dict(_5=None), dict(_9=None, _11=None)):
+        assert call(**change) == -1, change
+
+
+def _drafts(**change):
+    a = dict(target_probs=torch.zeros(2, 4, 10), draft_tokens=torch.zeros(2, 3, dtype=torch.int64), uniforms=torch.zeros(2, 4),
+             draft_probs=torch.zeros(2, 3, 10), num_drafts=torch.zeros(2, dtype=torch.int64))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(target_probs=torch.zeros(2, 4, 10).half()), dict(target_probs=torch.zeros(2, 10)), dict(target_probs=torch.zeros(2, 4, 0)),
+    dict(target_probs=torch.zeros(2, 0, 10)), dict(draft_tokens=torch.zeros(2, 4, dtype=torch.int64)),
+    dict(draft_tokens=torch.zeros(2, 3, dtype=torch.int32)), dict(uniforms=torch.zeros(2, 3)), dict(uniforms=torch.zeros(2, 4).double()),
+    dict(draft_probs=torch.zeros(2, 4, 10)), dict(draft_probs=torch.zeros(2, 3, 10).bfloat16()),
+    dict(num_drafts=torch.zeros(3, dtype=torch.int64)), dict(num_drafts=torch.zeros(2, dtype=torch.int32)), {}])
+def test_verify_refusals(change):
+    with pytest.raises(ValueError, match="CUDA" if not change else "^verify: "):
+        verify.verify_drafts(**_drafts(**change))
+    with pytest.raises(ValueError):
+        verify.run(_drafts(**change))
+
+
+def test_verify_abi_refusals():
+    fn = _native.load("verify").ckb_verify_launch
+    p = 16
+    good = [p, p, p, None, p, p, p, 40, 10, 30, 10, 2, 3, 10, 0, None]
+    assert fn(*good[:11], 0, *good[12:]) == 0
+    for i, v in ((0, None), (2, None), (4, None), (5, None), (6, None), (11, 1 << 31), (12, -1), (12, 1 << 20), (13, 0),
+                 (13, (1 << 30) + 1), (14, 2), (14, -1)):
+        assert fn(*good[:i], v, *good[i + 1:]) == -1, (i, v)
+
+
+def test_the_oracle_of_the_verification_is_the_definition():
+    target = torch.tensor([[[0.5, 0.25, 0.25], [0.0, 0.5, 0.5]]])
+    draft = torch.tensor([[[0.25, 0.75, 0.0]]])
+    tok = torch.tensor([[1]])
+    assert serving.verify(target, tok, torch.tensor([[0.3, 0.4]]), draft)[0].tolist() == [[1, 1]]  # .3 * .75 < .25
+    assert serving.verify(target, tok, torch.tensor([[0.4, 0.4]]), draft)[0].tolist() == [[0, -1]]  # w = (.25, 0, .25)
+    assert serving.verify(target, tok, torch.tensor([[0.4, 0.5]]), draft)[0].tolist() == [[2, -1]]
+    assert serving.verify(target, tok, torch.tensor([[0.3, 0.4]]))[0].tolist() == [[0, -1]]  # one-hot: .3 >= .25
