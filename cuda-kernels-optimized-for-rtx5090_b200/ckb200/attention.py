@@ -1,0 +1,99 @@
+"""Paged attention on B200: run({"q", "key_cache", "value_cache", "block_tables", "seq_lens"[, "scale", "shared_prefix"]})
+-> {"out"}.
+
+The attention of a decoding step over the cache that rope.rope_kv_cache and rope.qk_norm_rope_kv_cache write: one new token
+of each sequence, or several drafted ones, grouped query heads, and a prefix (a system prompt, a document) that all
+sequences of the batch share and that is then read once for the whole batch. No counterpart in the reference; the
+library's C entry is ckb_attention_paged_launch.
+"""
+
+import ctypes
+
+import torch
+
+from . import _native
+
+_DTYPES = {torch.bfloat16: 1, torch.float16: 2}
+_STRIDES = ctypes.c_longlong * 3
+
+
+def _problem(q, key_cache, value_cache, tables, lens, prefix):
+    """Why these inputs are not an attention these kernels serve, or None."""
+    if q.dtype not in _DTYPES or q.dim() != 4 or min(q.shape[1:]) < 1:
+        return f"q {q.dtype} {tuple(q.shape)}, bf16 or fp16 [B, T, Hq, D] is served"
+    batch, _, q_heads, head_dim = q.shape
+    if head_dim % 8 or head_dim > 256:
+        return f"head_dim {head_dim}, a multiple of 8 up to 256 is served"
+    for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
+        if c.dtype != q.dtype or c.dim() != 4 or c.shape[3] != head_dim or c.shape[1] < 1 or c.shape[2] < 1 or \
+                not c.is_contiguous():
+            return (f"{name} must be a contiguous [blocks, block_size, Hkv, {head_dim}] tensor of {q.dtype}, got {c.dtype} "
+                    f"{tuple(c.shape)}")
+    if key_cache.shape != value_cache.shape:
+        return f"key_cache {tuple(key_cache.shape)} and value_cache {tuple(value_cache.shape)} differ"
+    if q_heads % key_cache.shape[2]:
+        return f"{q_heads} query heads for {key_cache.shape[2]} key heads"
+    if tables.dtype != torch.int64 or tables.dim() != 2 or tables.shape[0] != batch or tables.shape[1] < 1:
+        return f"block_tables {tables.dtype} {tuple(tables.shape)}, int64 [{batch}, blocks] is needed"
+    if lens.dtype != torch.int64 or tuple(lens.shape) != (batch,):
+        return f"seq_lens {lens.dtype} {tuple(lens.shape)}, int64 [{batch}] is needed"
+    block_size = key_cache.shape[1]
+    if not isinstance(prefix, int) or prefix < 0 or prefix % block_size or prefix > tables.shape[1] * block_size:
+        return (f"shared_prefix {prefix!r} must be a number of tokens, a multiple of the block size {block_size}, within the "
+                f"{tables.shape[1]} blocks of a sequence")
+    return None
+
+
+def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=None, shared_prefix=0, out=None):
+    """softmax(scale * q k^T) v over each sequence's cached tokens: [B, T, Hq, D] in q's dtype.
+
+    q [B, T, Hq, D] (bf16 or fp16, any strides with a contiguous last dim, so a view of a fused projection) holds the T
+    newest tokens of each sequence, whose keys and values are in the cache already; key_cache / value_cache [num_blocks,
+    block_size, Hkv, D] in the same dtype; block_tables [B, M] int64, the blocks of each sequence in order; seq_lens [B]
+    int64, the tokens of each sequence with the T new ones. Token t sees the positions below seq_lens - T + t + 1; with
+    none (a padded row of the batch: length 0) its output is zeros. scale defaults to D ** -0.5. shared_prefix: the number
+    of tokens (a multiple of block_size) with which every sequence begins in the SAME blocks; they are read once, through
+    row 0 of block_tables. A block id outside the cache reads as zeros. Scores, softmax statistics and sums are fp32."""
+    problem = _problem(q, key_cache, value_cache, block_tables, seq_lens, shared_prefix)
+    if problem:
+        raise ValueError(f"attention: {problem}")
+    batch, tokens, q_heads, head_dim = q.shape
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"attention: scale must be a positive finite number, got {scale}")
+    _native.require_cuda("attention", q, key_cache, value_cache, block_tables, seq_lens)
+    if key_cache.data_ptr() % 16 or value_cache.data_ptr() % 16:
+        raise ValueError("attention: the caches must start on 16-byte boundaries")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device or \
+            out.data_ptr() % 16:
+        raise ValueError("attention: out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
+    if batch == 0:
+        return out
+    strides = [0 if n == 1 else st for n, st in zip(q.shape[:3], q.stride()[:3])]
+    if q.stride(3) != 1 or q.data_ptr() % 16 or any(st % 8 for st in strides):
+        q = q.clone(memory_format=torch.contiguous_format)
+        strides = q.stride()[:3]
+    tables, lens = block_tables.contiguous(), seq_lens.contiguous()
+    num_blocks, block_size, kv_heads, _ = key_cache.shape
+    lib = _native.load("attention")
+    with torch.cuda.device(q.device):
+        sizes = (batch, tokens, q_heads, kv_heads, head_dim, block_size, tables.shape[1], shared_prefix)
+        need = lib.ckb_attention_workspace(*sizes)
+        if need < 0:
+            raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
+                             f"block_tables {tuple(tables.shape)}")
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        err = lib.ckb_attention_paged_launch(q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), tables.data_ptr(),
+                                             lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES(*strides),
+                                             batch, tokens, q_heads, kv_heads, head_dim, num_blocks, block_size,
+                                             tables.shape[1], shared_prefix, scale, _DTYPES[q.dtype],
+                                             _native.stream_of(q))
+    _native.check(err)
+    return out
+
+
+def run(inputs):
+    return {"out": paged_attention(inputs["q"], inputs["key_cache"], inputs["value_cache"], inputs["block_tables"],
+                                   inputs["seq_lens"], inputs.get("scale"), inputs.get("shared_prefix", 0))}

@@ -18,7 +18,7 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_ROOT = os.path.join(PKG_ROOT, "lib")
 OPS = ("softmax", "rmsnorm", "rope", "topk")
-SERVING_OPS = ("verify",)  # ops without a counterpart in the reference, under their own symbols
+SERVING_OPS = ("attention", "verify")  # ops without a counterpart in the reference, under their own symbols
 LIBS = OPS + SERVING_OPS
 
 NVCC_FLAGS = [

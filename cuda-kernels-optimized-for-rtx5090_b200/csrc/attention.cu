@@ -1,0 +1,772 @@
+// Attention of a few new tokens per sequence over a paged key/value cache, with a prefix that the whole batch shares.
+//
+// For query row (b, t, head h of its kv head's group), the positions j < L = lens[b] - T + t + 1, x_j = scale q.k_j:
+//   out = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),  m = max_j x_j
+// computed piece by piece: a piece of positions gives (m, l = sum exp(x - m), o = sum exp(x - m) v), and pieces join by
+//   M = max m_i,  out = sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i.
+// x, m, l and o are fp32; the weights exp(x - m) are rounded to the cache's dtype for the product with v (half a step of
+// that dtype on each, as the output's own rounding), q, k and v enter the products as they are.
+//
+// Two kinds of work, of tiles of kTile positions:
+//   own     the positions behind the prefix: a unit is (sequence, kv head, up to 64 of its T * group rows), its positions
+//           are the sequence's own. Bound by the bytes of the cache: every key and value is read once, by one CTA;
+//   shared  the prefix's positions: a unit is (kv head, rows of ALL sequences), so each key and value of the prefix is
+//           read once for many rows, not once for every sequence.
+// The tiles of all units are laid end to end and cut into equal runs, one for each CTA (the own lengths are only known on
+// the device: every CTA adds them up itself). So unequal lengths and few sequences fill the GPU alike. A run's part of a
+// unit is a piece; pieces go to the workspace at slot (unit + CTA), which is different for each, and join_rows joins
+// them. A whole unit, where no prefix is shared, is written out at once.
+#include "ckb200_attention.h"
+#include "common.cuh"
+
+#include <climits>
+
+namespace ckb {
+namespace {
+
+constexpr int kTile = 64;      // positions of a tile
+constexpr int kThreads = 128;  // four warps
+constexpr int kMaxBatch = 8192;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct View3 {
+  long long batch, token, head;
+};
+
+struct Args {
+  const void *q, *key, *value;
+  const long long *tables, *lens;
+  void* out;
+  float* part;     // [slots][rows of a tile][D] of this launch's pieces
+  float2* ml;      // [slots][rows of a tile]: (m in powers of 2, l)
+  int* plan;       // own work only: [batch + 1] running tile counts, then the tiles of a run
+  View3 vq;
+  long long num_blocks;
+  int batch, tokens, q_heads, kv_heads, group, head_dim, block_size, table_width;
+  int prefix;      // positions of the shared prefix
+  int rows;        // tokens * group: query rows of a sequence and kv head
+  int row_tiles;   // row tiles of a unit's rows
+  float scale_log2;
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// Tensor-core fragments (m16n8k16) and asynchronous copies.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void ldsm4_trans(unsigned (&r)[4], unsigned at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+// 16 bytes global -> shared; without `fill` the bytes are zeros and nothing is read.
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool fill) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of rows of DT 16-bit values: chunks are exchanged within a row so that
+// the 8 rows an ldmatrix reads lie in different banks.
+template <int DT>
+__device__ __forceinline__ unsigned at_chunk(int r, int c) {
+  return r * (DT * 2) + ((c ^ (r & 7)) << 4);
+}
+
+// Two neighbouring values of shared memory.
+__device__ __forceinline__ unsigned load_word(unsigned at) {
+  unsigned w;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+  return w;
+}
+__device__ __forceinline__ float2 load2(unsigned at, __nv_bfloat16) {
+  const unsigned w = load_word(at);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 load2(unsigned at, __half) {
+  const unsigned w = load_word(at);
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// Whether any value of rows row0 .. row0 + kCount - 1 of a tile is infinite or NaN (the whole warp asks).
+template <typename T, int DT, int kCount>
+__device__ __forceinline__ bool not_finite(unsigned tile, int row0, int lane) {
+  bool bad = false;
+#pragma unroll 4
+  for (int i = lane; i < kCount * (DT / 2); i += 32) {
+    const float2 v = load2(tile + row0 * (DT * 2) + i * 4, T{});
+    bad |= !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY);
+  }
+  return __any_sync(0xffffffffu, bad);
+}
+
+// The rows of a unit: row r of the tile is query (b, t, head), or nothing.
+struct Row {
+  int b, t, head;  // head: of the q heads
+  bool real;
+};
+template <bool kShared>
+__device__ __forceinline__ Row row_of(const Args& a, int b, int kv_head, int r) {
+  Row x;
+  x.real = r < (kShared ? a.batch * a.rows : a.rows);
+  x.b = kShared ? r / a.rows : b;
+  const int in = kShared ? r - x.b * a.rows : r;
+  x.t = in / a.group;
+  x.head = kv_head * a.group + (in - x.t * a.group);
+  return x;
+}
+__device__ __forceinline__ long long length_of(const Args& a, int b) {
+  const long long most = (long long)a.table_width * a.block_size, n = __ldg(a.lens + b);
+  return n < 0 ? 0 : n < most ? n : most;
+}
+// The positions that token t of sequence b sees: those below this (none if it is not positive).
+__device__ __forceinline__ int limit_of(const Args& a, int b, int t) {
+  return (int)length_of(a, b) - a.tokens + t + 1;
+}
+__device__ __forceinline__ int own_tiles(const Args& a, int b) {
+  const int own = (int)length_of(a, b) - a.prefix;
+  return own > 0 ? (own + kTile - 1) / kTile : 0;
+}
+
+// A place on the axis of tiles.
+struct Cursor {
+  int b, unit, tile, tiles;  // sequence (0 in shared work), unit within it, tile within the unit, the unit's tiles
+};
+
+template <typename T, int DT, int WR, bool kShared>
+struct Shape {
+  static constexpr int kRows = 16 * WR;        // query rows of a tile
+  static constexpr int kKeyWarps = 4 / WR;     // warps that share a tile's positions
+  static constexpr int kKeys = kTile / kKeyWarps;
+  static constexpr int kStages = WR == 1 && DT <= 128 ? 3 : 2;  // what leaves room for per_sm() CTAs
+  static constexpr int kTileBytes = kTile * DT * 2;
+  static constexpr int kQBytes = kRows * DT * 2;
+  static constexpr int kOffQ = kStages * 2 * kTileBytes;
+  static constexpr int kOffRows = kOffQ + kStages * kQBytes;  // units may be one tile long: a q buffer for each stage
+  static constexpr int kOffMl = kOffRows + 2 * kTile * 8;
+  static constexpr int kOffLimits = kOffMl + kKeyWarps * kRows * 8;
+  static constexpr int kOffCum = kOffLimits + kRows * 4;
+  static int bytes(int batch) { return kOffCum + (kShared ? 2 : batch + 1) * 4; }
+};
+
+template <typename T, int DT, int WR, bool kShared>
+__global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
+  using S = Shape<T, DT, WR, kShared>;
+  constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages;
+  constexpr int kChunks = DT / 8;                // 16-byte chunks of a row
+  constexpr int kRowsPerPass = kThreads / kChunks;
+  extern __shared__ __align__(128) unsigned char smem[];
+  long long* row_at = reinterpret_cast<long long*>(smem + S::kOffRows);  // [2][kTile] cache rows, -1: zeros
+  float2* ml_sh = reinterpret_cast<float2*>(smem + S::kOffMl);           // [key warps][rows]
+  int* limits = reinterpret_cast<int*>(smem + S::kOffLimits);
+  int* cum = reinterpret_cast<int*>(smem + S::kOffCum);
+  const unsigned smem_at = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, wk = warp / WR;
+  pdl_wait();
+  pdl_trigger();
+
+  // The axis of tiles.
+  const int units = a.kv_heads * a.row_tiles;  // of a sequence
+  const int seqs = kShared ? 1 : a.batch;
+  if (kShared) {
+    if (tid == 0) {
+      cum[0] = 0;
+      cum[1] = units * ((a.prefix + kTile - 1) / kTile);
+    }
+  } else {
+    int* warp_tiles = reinterpret_cast<int*>(ml_sh);
+    int before = 0;
+    for (int base = 0; base < a.batch; base += kThreads) {
+      const int b = base + tid;
+      const int mine = b < a.batch ? own_tiles(a, b) * units : 0;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) warp_tiles[warp] = upto;
+      __syncthreads();
+      for (int k = 0; k < warp; ++k) upto += warp_tiles[k];
+      if (b < a.batch) cum[b] = before + upto - mine;
+      for (int k = 0; k < kThreads / 32; ++k) before += warp_tiles[k];
+      __syncthreads();
+    }
+    if (tid == 0) cum[a.batch] = before;
+  }
+  __syncthreads();
+  const int all = cum[seqs];
+  const int run = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
+  if (!kShared && blockIdx.x == 0) {
+    for (int b = tid; b <= a.batch; b += kThreads) a.plan[b] = cum[b];
+    if (tid == 0) a.plan[a.batch + 1] = run;
+  }
+  const int first = (int)min((long long)blockIdx.x * run, (long long)all);
+  const int last = min(first + run, all);
+  if (first >= last) return;
+
+  const auto start = [&](int w) {
+    int lo = 0, hi = seqs;  // the last b with cum[b] <= w
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cum[mid] <= w) lo = mid;
+      else hi = mid;
+    }
+    Cursor c;
+    c.b = lo;
+    c.tiles = (cum[lo + 1] - cum[lo]) / units;
+    c.unit = (w - cum[lo]) / c.tiles;
+    c.tile = w - cum[lo] - c.unit * c.tiles;
+    return c;
+  };
+  const auto next = [&](Cursor& c) {  // never past the axis: callers stop at `last`
+    if (++c.tile < c.tiles) return;
+    c.tile = 0;
+    if (++c.unit < units) return;
+    c.unit = 0;
+    do {
+      ++c.b;
+      c.tiles = c.b < seqs ? (cum[c.b + 1] - cum[c.b]) / units : 1;
+    } while (c.b < seqs && c.tiles == 0);
+  };
+  // The cache row of position (tile, lane of the tile), or -1.
+  const auto lookup = [&](const Cursor& c, int i) -> long long {
+    const int pos = (kShared ? 0 : a.prefix) + c.tile * kTile + i;
+    const int end = kShared ? a.prefix : (int)length_of(a, c.b);
+    if (pos >= end) return -1;
+    const int page = pos / a.block_size;
+    const long long block = __ldg(a.tables + (kShared ? 0LL : (long long)c.b * a.table_width) + page);
+    if (block < 0 || block >= a.num_blocks) return -1;
+    return block * a.block_size + (pos - page * a.block_size);
+  };
+  const auto issue = [&](const Cursor& c, int stage, int slot, int q_buffer, bool with_q) {
+    const int kv_head = c.unit / a.row_tiles, chunk = tid % kChunks;
+    const bool inside = chunk * 8 < a.head_dim;
+    const unsigned k_at = smem_at + stage * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
+#pragma unroll
+    for (int p = 0; p < kTile / kRowsPerPass; ++p) {
+      const int r = p * kRowsPerPass + tid / kChunks;
+      const long long row = row_at[slot * kTile + r];
+      const bool fill = inside && row >= 0;
+      const long long off = fill ? (row * a.kv_heads + kv_head) * a.head_dim + chunk * 8 : 0;
+      copy16(k_at + at_chunk<DT>(r, chunk), (const T*)a.key + off, fill);
+      copy16(v_at + at_chunk<DT>(r, chunk), (const T*)a.value + off, fill);
+    }
+    if (with_q) {
+      const int row0 = (c.unit - kv_head * a.row_tiles) * kRows;
+      for (int r = tid / kChunks; r < kRows; r += kRowsPerPass) {
+        const Row x = row_of<kShared>(a, c.b, kv_head, row0 + r);
+        const bool fill = inside && x.real;
+        const long long off = fill ? x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head + chunk * 8 : 0;
+        copy16(smem_at + S::kOffQ + q_buffer * S::kQBytes + at_chunk<DT>(r, chunk), (const T*)a.q + off, fill);
+      }
+    }
+  };
+
+  // Three cursors run along the axis: page look-ups kStages tiles ahead, copies kStages - 1 ahead, the products.
+  Cursor look = start(first), load = look, at = look;
+  int looked = first, loaded = first, q_loads = 0;
+  const auto look_and_store = [&]() {
+    if (looked >= last) return;
+    if (tid < kTile) row_at[(looked & 1) * kTile + tid] = lookup(look, tid);
+    next(look);
+    ++looked;
+  };
+  const auto load_one = [&]() {
+    if (loaded < last) {
+      const bool with_q = loaded == first || load.tile == 0;
+      if (with_q) ++q_loads;
+      issue(load, (loaded - first) % kStages, loaded & 1, q_loads % kStages, with_q);
+      next(load);
+      ++loaded;
+    }
+    copy_commit();
+  };
+  look_and_store();
+  for (int i = 0; i < kStages - 1; ++i) {
+    __syncthreads();
+    load_one();
+    look_and_store();
+  }
+
+  constexpr int kNt = kKeys / 8;   // score tiles of 8 positions
+  constexpr int kDt = DT / 8;      // output tiles of 8 columns
+  float o[kDt][4], m[2], l[2];
+  int min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
+  const int quad_row = lane >> 2;
+  for (int w = first; w < last; ++w) {
+    copy_wait<kStages - 2>();
+    __syncthreads();  // tile w is there for all, tile w - 1's stage is free
+    load_one();
+    long long next_row = -1;
+    const bool looking = looked < last;
+    if (looking && tid < kTile) next_row = lookup(look, tid);
+
+    const int kv_head = at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
+    if (w == first || at.tile == 0) {  // a new piece
+      ++q_now;
+      piece_begin = at.tile;
+      if (tid < kRows) {
+        const Row x = row_of<kShared>(a, at.b, kv_head, row0 + tid);
+        const int n = x.real ? max(0, limit_of(a, x.b, x.t)) : INT_MAX;  // a row of padding: any finite result
+        limits[tid] = kShared ? min(n, a.prefix) : n;
+      }
+      __syncthreads();
+      min_limit = INT_MAX;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) min_limit = min(min_limit, limits[wr * 16 + r]);
+      lim[0] = limits[wr * 16 + quad_row];
+      lim[1] = limits[wr * 16 + quad_row + 8];
+#pragma unroll
+      for (int n = 0; n < kDt; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.0f;
+    }
+
+    const unsigned k_at = smem_at + ((w - first) % kStages) * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
+    const unsigned q_at = smem_at + S::kOffQ + (q_now % kStages) * S::kQBytes;
+    const int pos0 = (kShared ? 0 : a.prefix) + at.tile * kTile + wk * kKeys;
+    float s[kNt][4];
+#pragma unroll
+    for (int n = 0; n < kNt; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DT / 16; ++k) {
+      unsigned qa[4];
+      ldsm4(qa, q_at + at_chunk<DT>(wr * 16 + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+      for (int n = 0; n < kNt; n += 2) {
+        unsigned kb[4];
+        ldsm4(kb, k_at + at_chunk<DT>(wk * kKeys + n * 8 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
+        mma(s[n], qa, kb[0], kb[1], T{});
+        mma(s[n + 1], qa, kb[2], kb[3], T{});
+      }
+    }
+    const bool masked = pos0 + kKeys > min_limit;
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (pos0 + n * 8 + (lane & 3) * 2 + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
+    }
+    float scale_o[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float top = m[i];
+#pragma unroll
+      for (int n = 0; n < kNt; ++n) top = fmaxf(top, fmaxf(s[n][2 * i], s[n][2 * i + 1]) * a.scale_log2);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float ref = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      scale_o[i] = exp2_fast(m[i] - ref);
+      m[i] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = exp2_fast(fmaf(s[n][2 * i + e], a.scale_log2, -ref));
+          s[n][2 * i + e] = p;
+          sum += p;
+        }
+      l[i] = l[i] * scale_o[i] + sum;
+    }
+#pragma unroll
+    for (int n = 0; n < kDt; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] *= scale_o[e >> 1];
+    if (masked && not_finite<T, DT, kKeys>(v_at, wk * kKeys, lane)) {
+      // A value that some row must not see is not finite: 0 * v would carry it over. One position after the other.
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+        for (int j = 0; j < 8; ++j) {
+          const int key = n * 8 + j, from = (lane & ~3) | (j >> 1);
+          const float p0 = round_through<T>(__shfl_sync(0xffffffffu, j & 1 ? s[n][1] : s[n][0], from));
+          const float p1 = round_through<T>(__shfl_sync(0xffffffffu, j & 1 ? s[n][3] : s[n][2], from));
+          const bool see0 = pos0 + key < lim[0], see1 = pos0 + key < lim[1];
+#pragma unroll
+          for (int c = 0; c < kDt; ++c) {
+            const float2 v = load2(v_at + at_chunk<DT>(wk * kKeys + key, c) + (lane & 3) * 4, T{});
+            if (see0) {
+              o[c][0] = fmaf(p0, v.x, o[c][0]);
+              o[c][1] = fmaf(p0, v.y, o[c][1]);
+            }
+            if (see1) {
+              o[c][2] = fmaf(p1, v.x, o[c][2]);
+              o[c][3] = fmaf(p1, v.y, o[c][3]);
+            }
+          }
+        }
+    } else
+#pragma unroll
+    for (int k = 0; k < kKeys / 16; ++k) {
+      unsigned pa[4];
+      pa[0] = pack2(s[2 * k][0], s[2 * k][1], T{});
+      pa[1] = pack2(s[2 * k][2], s[2 * k][3], T{});
+      pa[2] = pack2(s[2 * k + 1][0], s[2 * k + 1][1], T{});
+      pa[3] = pack2(s[2 * k + 1][2], s[2 * k + 1][3], T{});
+#pragma unroll
+      for (int n = 0; n < kDt; n += 2) {
+        unsigned vb[4];
+        ldsm4_trans(vb, v_at + at_chunk<DT>(wk * kKeys + k * 16 + (lane & 15), n + (lane >> 4)));
+        mma(o[n], pa, vb[0], vb[1], T{});
+        mma(o[n + 1], pa, vb[2], vb[3], T{});
+      }
+    }
+
+    if (at.tile + 1 == at.tiles || w + 1 == last) {  // the end of a piece
+      const bool whole = !kShared && a.prefix == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
+      const long long slot = (long long)at.b * units + at.unit + blockIdx.x;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      if (S::kKeyWarps > 1) {  // join the warps that shared the positions, in the tile's own stage
+        if ((lane & 3) == 0) {
+          ml_sh[wk * kRows + wr * 16 + quad_row] = make_float2(m[0], l[0]);
+          ml_sh[wk * kRows + wr * 16 + quad_row + 8] = make_float2(m[1], l[1]);
+        }
+        __syncthreads();  // and nobody reads the tile any more
+        float* sum_o = reinterpret_cast<float*>(smem + ((w - first) % kStages) * 2 * S::kTileBytes);
+        float weight[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = wr * 16 + quad_row + 8 * i;
+          const float mine = m[i];
+          float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) top = fmaxf(top, ml_sh[k * kRows + r].x);
+          const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) sum += ml_sh[k * kRows + r].y * exp2_fast(ml_sh[k * kRows + r].x - ref);
+          weight[i] = exp2_fast(mine - ref);
+          m[i] = top;
+          l[i] = sum;
+        }
+        for (int k = 0; k < S::kKeyWarps; ++k) {
+          if (wk == k) {
+#pragma unroll
+            for (int n = 0; n < kDt; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float2* dst = reinterpret_cast<float2*>(sum_o + (wr * 16 + quad_row + 8 * i) * DT + n * 8 + (lane & 3) * 2);
+                float2 v = make_float2(o[n][2 * i] * weight[i], o[n][2 * i + 1] * weight[i]);
+                if (k > 0) {
+                  const float2 u = *dst;
+                  v.x += u.x;
+                  v.y += u.y;
+                }
+                *dst = v;
+                o[n][2 * i] = v.x;
+                o[n][2 * i + 1] = v.y;
+              }
+          }
+          __syncthreads();
+        }
+      }
+      if (wk == S::kKeyWarps - 1) {  // the last to add holds the sums
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = wr * 16 + quad_row + 8 * i;
+          const Row x = row_of<kShared>(a, at.b, kv_head, row0 + r);
+          if (!x.real) continue;
+          if (whole) {
+            const float inv = lim[i] > 0 ? 1.0f / l[i] : 0.0f;
+            T* dst = (T*)a.out + (((long long)x.b * a.tokens + x.t) * a.q_heads + x.head) * a.head_dim;
+#pragma unroll
+            for (int n = 0; n < kDt; ++n) {
+              const int c = n * 8 + (lane & 3) * 2;
+              if (c < a.head_dim)
+                *reinterpret_cast<unsigned*>(dst + c) =
+                    lim[i] > 0 ? pack2(o[n][2 * i] * inv, o[n][2 * i + 1] * inv, T{}) : 0u;
+            }
+          } else {
+            float* dst = a.part + (slot * kRows + r) * a.head_dim;
+#pragma unroll
+            for (int n = 0; n < kDt; ++n) {
+              const int c = n * 8 + (lane & 3) * 2;
+              if (c < a.head_dim) *reinterpret_cast<float2*>(dst + c) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            }
+            if ((lane & 3) == 0) a.ml[slot * kRows + r] = make_float2(m[i], l[i]);
+          }
+        }
+      }
+    }
+    next(at);
+    if (looking) {
+      if (tid < kTile) row_at[(looked & 1) * kTile + tid] = next_row;
+      next(look);
+      ++looked;
+    }
+  }
+  copy_wait<0>();
+}
+
+// Joins the pieces of each output row: a warp per row (b, t, head).
+struct JoinArgs {
+  void* out;
+  const long long* lens;
+  const float *own_part, *shared_part;
+  const float2 *own_ml, *shared_ml;
+  const int* plan;
+  int batch, tokens, q_heads, kv_heads, group, head_dim, prefix, rows, table_positions;
+  int own_rows, own_row_tiles;        // rows of an own slot, row tiles of an own unit
+  int shared_rows, shared_row_tiles;  // the same of the shared work (0: none)
+  int shared_tiles, shared_run;       // tiles of a shared unit, tiles of a run
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (long long)a.batch * a.tokens * a.q_heads) return;
+  const int head = (int)(row % a.q_heads), t = (int)(row / a.q_heads % a.tokens), b = (int)(row / a.q_heads / a.tokens);
+  const int kv_head = head / a.group, in = t * a.group + (head - kv_head * a.group);
+
+  // Own pieces: slots own_slot, own_slot + 1, ...; shared ones the same.
+  const int units = a.kv_heads * a.own_row_tiles, unit = kv_head * a.own_row_tiles + in / a.own_rows;
+  const int begin = a.plan[b], tiles = (a.plan[b + 1] - begin) / units, run = a.plan[a.batch + 1];
+  int own = 0;
+  long long own_slot = 0;
+  if (tiles > 0) {
+    const int w0 = begin + unit * tiles, c0 = w0 / run;
+    own = (w0 + tiles - 1) / run - c0 + 1;
+    own_slot = (long long)b * units + unit + c0;
+    if (own == 1 && a.prefix == 0) return;  // written out by its CTA
+  }
+  int shared = 0;
+  long long shared_slot = 0;
+  const int all_row = b * a.rows + in;
+  if (a.shared_row_tiles > 0) {
+    const int u = kv_head * a.shared_row_tiles + all_row / a.shared_rows, w0 = u * a.shared_tiles, c0 = w0 / a.shared_run;
+    shared = (w0 + a.shared_tiles - 1) / a.shared_run - c0 + 1;
+    shared_slot = u + c0;
+  }
+  const long long own_at = own_slot * a.own_rows + in % a.own_rows;
+  const long long shared_at = a.shared_row_tiles > 0 ? shared_slot * a.shared_rows + all_row % a.shared_rows : 0;
+  const auto at = [&](int i) { return i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * a.shared_rows; };
+  const int pieces = own + shared;
+  float top = -INFINITY;
+  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, (i < own ? a.own_ml : a.shared_ml)[at(i)].x);
+  top = warp_max(top);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int i = lane; i < pieces; i += 32) {
+    const float2 v = (i < own ? a.own_ml : a.shared_ml)[at(i)];
+    sum += v.y * exp2_fast(v.x - ref);
+  }
+  sum = warp_sum(sum);
+  const long long n = a.lens[b], most = n < 0 ? 0 : n < a.table_positions ? n : a.table_positions;
+  const bool some = most - a.tokens + t + 1 > 0;
+  T* out = (T*)a.out + row * a.head_dim;
+  for (int c = lane * 4; c < a.head_dim; c += 128) {
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (some) {
+#pragma unroll 4
+      for (int i = 0; i < pieces; ++i) {
+        const float w = exp2_fast((i < own ? a.own_ml : a.shared_ml)[at(i)].x - ref);
+        const float4 v = *reinterpret_cast<const float4*>((i < own ? a.own_part : a.shared_part) + at(i) * a.head_dim + c);
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
+      }
+      const float inv = 1.0f / sum;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2(acc.x, acc.y, T{}), pack2(acc.z, acc.w, T{}));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------------------------------------------
+struct Sizes {
+  int rows, own_warps, own_rows, own_row_tiles, own_ctas;
+  int shared_row_tiles, shared_tiles, shared_ctas, shared_run;
+  long long own_slots, shared_slots, off_plan, off_own_ml, off_own, off_shared_ml, off_shared, bytes;
+};
+
+// CTAs of attend_tiles on an SM, by shared memory: 2 or 3 stages of 16, 32 or 64 KB for head_dim up to 64, 128 and 256.
+int per_sm(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1; }
+
+bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_dim, int block_size, long long table_width,
+              long long prefix, Sizes& z) {
+  if (batch < 1 || batch > kMaxBatch || tokens < 1 || tokens > 65536 || q_heads < 1 || kv_heads < 1 ||
+      q_heads > 65536 || q_heads % kv_heads || head_dim < 8 || head_dim > 256 || head_dim % 8 || block_size < 1 ||
+      table_width < 1 || prefix < 0 || prefix % block_size || table_width > INT_MAX / block_size - kTile ||
+      prefix > table_width * block_size)
+    return false;
+  const long long rows = (long long)tokens * (q_heads / kv_heads);
+  if (rows * batch * kv_heads > (1 << 26)) return false;
+  if (batch == 1) prefix = 0;  // nobody to share it with
+  z = Sizes{};
+  z.rows = (int)rows;
+  z.own_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  z.own_rows = 16 * z.own_warps;
+  z.own_row_tiles = (int)((rows + z.own_rows - 1) / z.own_rows);
+  const long long tiles = (table_width * block_size + kTile - 1) / kTile;
+  if (tiles * batch * kv_heads * z.own_row_tiles > INT_MAX / 2) return false;
+  const int most = device_sm_count() * per_sm(head_dim);
+  z.own_ctas = most;
+  z.own_slots = batch * kv_heads * z.own_row_tiles + z.own_ctas;
+  if (prefix > 0) {
+    z.shared_row_tiles = (int)((rows * batch + 63) / 64);
+    z.shared_tiles = (int)((prefix + kTile - 1) / kTile);
+    const long long all = (long long)z.shared_tiles * kv_heads * z.shared_row_tiles;
+    if (all > INT_MAX / 2) return false;
+    z.shared_ctas = (int)(all < most ? all : most);
+    z.shared_run = (int)((all + z.shared_ctas - 1) / z.shared_ctas);
+    z.shared_slots = (long long)kv_heads * z.shared_row_tiles + z.shared_ctas;
+  }
+  const auto up = [](long long n) { return (n + 255) / 256 * 256; };
+  z.off_plan = 0;
+  z.off_own_ml = up((batch + 2) * 4);
+  z.off_own = z.off_own_ml + up(z.own_slots * z.own_rows * 8);
+  z.off_shared_ml = z.off_own + up(z.own_slots * z.own_rows * head_dim * 4);
+  z.off_shared = z.off_shared_ml + up(z.shared_slots * 64 * 8);
+  z.bytes = z.off_shared + up(z.shared_slots * 64 * head_dim * 4);
+  return true;
+}
+
+template <typename T, int DT, int WR, bool kShared>
+cudaError_t start(const Args& a, int ctas, cudaStream_t stream) {
+  using S = Shape<T, DT, WR, kShared>;
+  const int bytes = S::bytes(a.batch);
+  const cudaError_t err = cudaFuncSetAttribute(attend_tiles<T, DT, WR, kShared>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(attend_tiles<T, DT, WR, kShared>, dim3(ctas), dim3(kThreads), bytes, stream, a);
+}
+
+template <typename T, int DT>
+cudaError_t start_own(const Args& a, int warps, int ctas, cudaStream_t stream) {
+  if (warps == 1) return start<T, DT, 1, false>(a, ctas, stream);
+  if (warps == 2) return start<T, DT, 2, false>(a, ctas, stream);
+  return start<T, DT, 4, false>(a, ctas, stream);
+}
+
+template <typename T>
+int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) {
+  const int dt = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+  cudaError_t err = cudaSuccess;
+  Args s = a;
+  a.row_tiles = z.own_row_tiles;
+  a.part = reinterpret_cast<float*>(work + z.off_own);
+  a.ml = reinterpret_cast<float2*>(work + z.off_own_ml);
+  s.row_tiles = z.shared_row_tiles;
+  s.part = reinterpret_cast<float*>(work + z.off_shared);
+  s.ml = reinterpret_cast<float2*>(work + z.off_shared_ml);
+  if (a.prefix > 0) {
+    err = dt == 64 ? start<T, 64, 4, true>(s, z.shared_ctas, stream)
+          : dt == 128 ? start<T, 128, 4, true>(s, z.shared_ctas, stream)
+                      : start<T, 256, 4, true>(s, z.shared_ctas, stream);
+  }
+  if (err == cudaSuccess)
+    err = dt == 64 ? start_own<T, 64>(a, z.own_warps, z.own_ctas, stream)
+          : dt == 128 ? start_own<T, 128>(a, z.own_warps, z.own_ctas, stream)
+                      : start_own<T, 256>(a, z.own_warps, z.own_ctas, stream);
+  if (err == cudaSuccess) {
+    const JoinArgs j{a.out, a.lens, a.part, s.part, a.ml, s.ml, a.plan, a.batch, a.tokens, a.q_heads, a.kv_heads, a.group,
+                     a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, 64,
+                     z.shared_row_tiles, z.shared_tiles, z.shared_run};
+    const long long rows = (long long)a.batch * a.tokens * a.q_heads;
+    err = launch_pdl(join_rows<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, j);
+  }
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return (int)err;
+  }
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ckb
+
+using namespace ckb;
+
+CKB_EXPORT long long ckb_attention_workspace(long long batch, int tokens, int q_heads, int kv_heads, int head_dim,
+                                             int block_size, long long table_width, long long shared_prefix) {
+  Sizes z;
+  return sizes_of(batch, tokens, q_heads, kv_heads, head_dim, block_size, table_width, shared_prefix, z) ? z.bytes : -1;
+}
+
+CKB_EXPORT int ckb_attention_paged_launch(const void* q, const void* key_cache, const void* value_cache,
+                                          const void* tables, const void* lens, void* out, void* work,
+                                          long long work_bytes, const long long* q_strides, long long batch, int tokens,
+                                          int q_heads, int kv_heads, int head_dim, long long num_blocks, int block_size,
+                                          long long table_width, long long shared_prefix, float scale, int dtype,
+                                          cudaStream_t stream) {
+  if (batch <= 0) return 0;
+  Sizes z;
+  if (!sizes_of(batch, tokens, q_heads, kv_heads, head_dim, block_size, table_width, shared_prefix, z)) return -1;
+  if (q == nullptr || tables == nullptr || lens == nullptr || out == nullptr || work == nullptr || q_strides == nullptr ||
+      num_blocks < 0 || (num_blocks > 0 && (key_cache == nullptr || value_cache == nullptr)) || work_bytes < z.bytes ||
+      !aligned16(q) || !aligned16(key_cache) || !aligned16(value_cache) || !aligned16(out) || !aligned16(work) ||
+      q_strides[0] % 8 || q_strides[1] % 8 || q_strides[2] % 8 || !(scale > 0.0f) || scale > 1e30f)
+    return -1;
+  unsigned char* w = static_cast<unsigned char*>(work);
+  Args a{};
+  a.q = q;
+  a.key = key_cache;
+  a.value = value_cache;
+  a.tables = static_cast<const long long*>(tables);
+  a.lens = static_cast<const long long*>(lens);
+  a.out = out;
+  a.plan = reinterpret_cast<int*>(w + z.off_plan);
+  a.vq = View3{q_strides[0], q_strides[1], q_strides[2]};
+  a.num_blocks = num_blocks;
+  a.batch = (int)batch;
+  a.tokens = tokens;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.head_dim = head_dim;
+  a.block_size = block_size;
+  a.table_width = (int)table_width;
+  a.prefix = batch == 1 ? 0 : (int)shared_prefix;
+  a.rows = z.rows;
+  a.scale_log2 = scale * kLog2e;
+  if (dtype == kBF16) return start_all<__nv_bfloat16>(a, z, w, stream);
+  if (dtype == kF16) return start_all<__half>(a, z, w, stream);
+  return -1;
+}

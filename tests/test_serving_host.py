@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from ckb200 import _native, build, rope, verify
+from ckb200 import _native, attention, build, rope, verify
 from oracle import serving
 from test_abi import declared
 
@@ -89,6 +89,77 @@ def test_qk_norm_abi_refusals():
                    dict(_17=1 << 20, _18=1 << 20), dict(_19=0), dict(_20=0), dict(_21=63), dict(_21=0), dict(_22=0),
                    dict(_22=3), dict(_23=3), dict(_24=-1), dict(_5=None), dict(_9=None, _11=None)):
         assert call(**change) == -1, change
+
+
+def _attend(**change):
+    a = dict(q=torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), key_cache=torch.zeros(9, 16, 2, 64, dtype=torch.bfloat16),
+             value_cache=torch.zeros(9, 16, 2, 64, dtype=torch.bfloat16), block_tables=torch.zeros(2, 4, dtype=torch.int64),
+             seq_lens=torch.zeros(2, dtype=torch.int64))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros(2, 3, 4, 64)), dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16)),
+    dict(q=torch.zeros(2, 0, 4, 64, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 3, 3, 64, dtype=torch.bfloat16)),
+    dict(q=torch.zeros(2, 3, 4, 60, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 3, 4, 264, dtype=torch.bfloat16)),
+    dict(key_cache=torch.zeros(9, 16, 2, 64).half()), dict(value_cache=torch.zeros(9, 16, 2, 128, dtype=torch.bfloat16)),
+    dict(value_cache=torch.zeros(8, 16, 2, 64, dtype=torch.bfloat16)),
+    dict(key_cache=torch.zeros(9, 2, 16, 64, dtype=torch.bfloat16).transpose(1, 2)),
+    dict(block_tables=torch.zeros(2, 4, dtype=torch.int32)), dict(block_tables=torch.zeros(3, 4, dtype=torch.int64)),
+    dict(block_tables=torch.zeros(2, 0, dtype=torch.int64)), dict(seq_lens=torch.zeros(2, dtype=torch.int32)),
+    dict(seq_lens=torch.zeros(2, 1, dtype=torch.int64)), dict(shared_prefix=8), dict(shared_prefix=-16),
+    dict(shared_prefix=80), dict(shared_prefix=16.0), dict(scale=0.0), dict(scale=float("nan")), dict(scale=-1.0), {}])
+def test_attention_refusals(change):
+    with pytest.raises(ValueError, match="CUDA" if not change else "^attention: "):
+        attention.paged_attention(**_attend(**change))
+    with pytest.raises(ValueError):
+        attention.run(_attend(**change))
+
+
+def test_attention_abi_refusals():
+    lib = _native.load("attention")
+    strides = (ctypes.c_longlong * 3)(768, 256, 64)
+    sizes = (2, 3, 4, 2, 64, 16, 4, 0)
+    need = lib.ckb_attention_workspace(*sizes)
+    assert need > 0
+    for i, v in ((0, 0), (0, 8193), (1, 0), (2, 3), (2, 0), (3, 0), (4, 0), (4, 12), (4, 264), (5, 0), (6, 0), (6, 1 << 40),
+                 (7, 8), (7, -16), (7, 80)):
+        assert lib.ckb_attention_workspace(*sizes[:i], v, *sizes[i + 1:]) == -1, (i, v)
+    assert lib.ckb_attention_workspace(1, 1, 32, 8, 128, 16, 8192, 0) < 64 << 20  # a long table costs nothing
+    p = 16
+    good = [p, p, p, p, p, p, p, need, strides, 2, 3, 4, 2, 64, 9, 16, 4, 0, 0.125, 1, None]
+    fn = lib.ckb_attention_paged_launch
+    assert fn(*good[:9], 0, *good[10:]) == 0
+    odd = (ctypes.c_longlong * 3)(768, 256, 60)
+    for i, v in ((0, None), (0, 8), (1, None), (1, 24), (2, 24), (3, None), (4, None), (5, None), (5, 8), (6, None), (6, 8),
+                 (7, need - 1), (8, None), (8, odd), (9, 8193), (10, 0), (11, 3), (13, 60), (14, -1), (15, 0), (16, 0),
+                 (17, 8), (18, 0.0), (18, -1.0), (18, float("nan")), (18, float("inf")), (19, 0), (19, 3)):
+        assert fn(*good[:i], v, *good[i + 1:]) == -1, (i, v)
+
+
+def test_attention_workspace_grows_with_the_batch_and_covers_the_prefix():
+    lib = _native.load("attention")
+    one = lib.ckb_attention_workspace(16, 1, 32, 8, 128, 16, 512, 0)
+    assert lib.ckb_attention_workspace(64, 1, 32, 8, 128, 16, 512, 0) > one
+    assert lib.ckb_attention_workspace(16, 1, 32, 8, 128, 16, 512, 4096) > one
+    assert lib.ckb_attention_workspace(1, 1, 32, 8, 128, 16, 512, 4096) == lib.ckb_attention_workspace(1, 1, 32, 8, 128, 16, 512, 0)
+
+
+def test_the_oracle_of_the_attention_is_torchs():
+    g = torch.Generator().manual_seed(1)
+    kc, vc = (torch.randn(6, 4, 2, 8, generator=g) for _ in range(2))
+    tables = torch.tensor([[3, 1, 0], [3, 5, 2]])
+    q = torch.randn(2, 2, 4, 8, generator=g)
+    for prefix in (0, 4):
+        got, _ = serving.attend(q, kc, vc, tables, torch.tensor([9, 6]), 0.3, prefix)
+        for b, n in enumerate((9, 6)):
+            k, v = (c[tables[b]].flatten(0, 1)[:n].repeat_interleave(2, 1).double() for c in (kc, vc))
+            for t in range(2):
+                m = n - 1 + t
+                want = torch.nn.functional.scaled_dot_product_attention(
+                    q[b, t][:, None].double(), k[:m].transpose(0, 1), v[:m].transpose(0, 1), scale=0.3)[:, 0]
+                torch.testing.assert_close(got[b, t], want)
 
 
 def _drafts(**change):
