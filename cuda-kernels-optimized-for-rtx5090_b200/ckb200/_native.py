@@ -52,6 +52,7 @@ SIGNATURES = {
         "ckb_attention_workspace": (_LL, [_LL] + [_INT] * 5 + [_LL] * 2),
         "ckb_attention_paged_launch": (_INT, [_VP] * 7 + [_LL, _VP, _LL] + [_INT] * 4 + [_LL, _INT, _LL, _LL, _FLT, _INT,
                                                                                        _VP]),
+        "ckb_attention_status": (_INT, [_INT]),
     },
     "verify": {
         "ckb_verify_launch": (_INT, [_VP] * 7 + [_LL] * 5 + [_INT] * 3 + [_VP]),

@@ -20,13 +20,14 @@
 #include "common.cuh"
 
 #include <climits>
+#include <type_traits>
 
 namespace ckb {
 namespace {
 
 constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
-constexpr int kMaxBatch = 8192;
+constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct View3 {
@@ -131,6 +132,15 @@ __device__ __forceinline__ bool not_finite(unsigned tile, int row0, int lane) {
   return __any_sync(0xffffffffu, bad);
 }
 
+// The same for a tile of 64-column halves.
+template <typename T, int DT, int kCount>
+__device__ __forceinline__ bool not_finite_box(unsigned tile, int row0, int lane) {
+  bool bad = false;
+#pragma unroll
+  for (int half = 0; half < DT / 64; ++half) bad |= not_finite<T, 64, kCount>(tile + half * (kTile * 128), row0, lane);
+  return bad;
+}
+
 // The rows of a unit: row r of the tile is query (b, t, head), or nothing.
 struct Row {
   int b, t, head;  // head: of the q heads
@@ -154,15 +164,93 @@ __device__ __forceinline__ long long length_of(const Args& a, int b) {
 __device__ __forceinline__ int limit_of(const Args& a, int b, int t) {
   return (int)length_of(a, b) - a.tokens + t + 1;
 }
-__device__ __forceinline__ int own_tiles(const Args& a, int b) {
-  const int own = (int)length_of(a, b) - a.prefix;
-  return own > 0 ? (own + kTile - 1) / kTile : 0;
-}
-
 // A place on the axis of tiles.
 struct Cursor {
   int b, unit, tile, tiles;  // sequence (0 in shared work), unit within it, tile within the unit, the unit's tiles
 };
+
+// The own work's axis: cum[b] tiles lie before sequence b, cum[batch] in all; lens[b] the clamped lengths. The whole block of
+// kCount threads takes part; `scratch` holds kCount / 32 ints.
+template <int kCount>
+__device__ __forceinline__ void own_axis(const Args& a, int units, int* cum, int* lens, int* scratch) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int before = 0;
+  for (int base = 0; base < a.batch; base += kCount) {
+    const int b = base + tid;
+    int mine = 0;
+    if (b < a.batch) {
+      const int len = (int)length_of(a, b);
+      lens[b] = len;
+      mine = len > a.prefix ? (len - a.prefix + kTile - 1) / kTile * units : 0;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) scratch[warp] = upto;
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) upto += scratch[k];
+    if (b < a.batch) cum[b] = before + upto - mine;
+    for (int k = 0; k < kCount / 32; ++k) before += scratch[k];
+    __syncthreads();
+  }
+  if (tid == 0) cum[a.batch] = before;
+  __syncthreads();
+}
+// Tile w of the axis of `seqs` sequences (w < cum[seqs]).
+__device__ __forceinline__ Cursor axis_start(const int* cum, int seqs, int units, int w) {
+  int lo = 0, hi = seqs;  // the last b with cum[b] <= w
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] <= w) lo = mid;
+    else hi = mid;
+  }
+  Cursor c;
+  c.b = lo;
+  c.tiles = (cum[lo + 1] - cum[lo]) / units;
+  c.unit = (w - cum[lo]) / c.tiles;
+  c.tile = w - cum[lo] - c.unit * c.tiles;
+  return c;
+}
+// The next tile. Past the axis' end the cursor names no tile (callers stop there).
+__device__ __forceinline__ void axis_next(const int* cum, int seqs, int units, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.unit < units) return;
+  c.unit = 0;
+  do {
+    ++c.b;
+    c.tiles = c.b < seqs ? (cum[c.b + 1] - cum[c.b]) / units : 1;
+  } while (c.b < seqs && c.tiles == 0);
+}
+
+// Writes a lane's part of row half i of an accumulator o: the output itself where the piece is the whole unit, else the
+// piece at workspace row `at`.
+template <typename T, int DT>
+__device__ __forceinline__ void write_row(const Args& a, const Row& x, bool whole, bool some, long long at, int lane,
+                                          const float (&o)[DT / 8][4], int i, float m, float l) {
+  if (!x.real) return;
+  if (whole) {
+    const float inv = 1.0f / l;
+    T* dst = (T*)a.out + (((long long)x.b * a.tokens + x.t) * a.q_heads + x.head) * a.head_dim;
+#pragma unroll
+    for (int n = 0; n < DT / 8; ++n) {
+      const int c = n * 8 + (lane & 3) * 2;
+      if (c < a.head_dim)
+        *reinterpret_cast<unsigned*>(dst + c) = some ? pack2(o[n][2 * i] * inv, o[n][2 * i + 1] * inv, T{}) : 0u;
+    }
+  } else {
+    float* dst = a.part + at * a.head_dim;
+#pragma unroll
+    for (int n = 0; n < DT / 8; ++n) {
+      const int c = n * 8 + (lane & 3) * 2;
+      if (c < a.head_dim) *reinterpret_cast<float2*>(dst + c) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+    if ((lane & 3) == 0) a.ml[at] = make_float2(m, l);
+  }
+}
 
 template <typename T, int DT, int WR, bool kShared>
 struct Shape {
@@ -177,7 +265,7 @@ struct Shape {
   static constexpr int kOffMl = kOffRows + 2 * kTile * 8;
   static constexpr int kOffLimits = kOffMl + kKeyWarps * kRows * 8;
   static constexpr int kOffCum = kOffLimits + kRows * 4;
-  static int bytes(int batch) { return kOffCum + (kShared ? 2 : batch + 1) * 4; }
+  static int bytes(int batch) { return kOffCum + (kShared ? 2 : 2 * batch + 1) * 4; }
 };
 
 template <typename T, int DT, int WR, bool kShared>
@@ -206,25 +294,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
       cum[1] = units * ((a.prefix + kTile - 1) / kTile);
     }
   } else {
-    int* warp_tiles = reinterpret_cast<int*>(ml_sh);
-    int before = 0;
-    for (int base = 0; base < a.batch; base += kThreads) {
-      const int b = base + tid;
-      const int mine = b < a.batch ? own_tiles(a, b) * units : 0;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      if (lane == 31) warp_tiles[warp] = upto;
-      __syncthreads();
-      for (int k = 0; k < warp; ++k) upto += warp_tiles[k];
-      if (b < a.batch) cum[b] = before + upto - mine;
-      for (int k = 0; k < kThreads / 32; ++k) before += warp_tiles[k];
-      __syncthreads();
-    }
-    if (tid == 0) cum[a.batch] = before;
+    own_axis<kThreads>(a, units, cum, cum + a.batch + 1, reinterpret_cast<int*>(ml_sh));
   }
   __syncthreads();
   const int all = cum[seqs];
@@ -237,34 +307,10 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   const int last = min(first + run, all);
   if (first >= last) return;
 
-  const auto start = [&](int w) {
-    int lo = 0, hi = seqs;  // the last b with cum[b] <= w
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= w) lo = mid;
-      else hi = mid;
-    }
-    Cursor c;
-    c.b = lo;
-    c.tiles = (cum[lo + 1] - cum[lo]) / units;
-    c.unit = (w - cum[lo]) / c.tiles;
-    c.tile = w - cum[lo] - c.unit * c.tiles;
-    return c;
-  };
-  const auto next = [&](Cursor& c) {  // never past the axis: callers stop at `last`
-    if (++c.tile < c.tiles) return;
-    c.tile = 0;
-    if (++c.unit < units) return;
-    c.unit = 0;
-    do {
-      ++c.b;
-      c.tiles = c.b < seqs ? (cum[c.b + 1] - cum[c.b]) / units : 1;
-    } while (c.b < seqs && c.tiles == 0);
-  };
   // The cache row of position (tile, lane of the tile), or -1.
   const auto lookup = [&](const Cursor& c, int i) -> long long {
     const int pos = (kShared ? 0 : a.prefix) + c.tile * kTile + i;
-    const int end = kShared ? a.prefix : (int)length_of(a, c.b);
+    const int end = kShared ? a.prefix : cum[a.batch + 1 + c.b];
     if (pos >= end) return -1;
     const int page = pos / a.block_size;
     const long long block = __ldg(a.tables + (kShared ? 0LL : (long long)c.b * a.table_width) + page);
@@ -296,12 +342,12 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   };
 
   // Three cursors run along the axis: page look-ups kStages tiles ahead, copies kStages - 1 ahead, the products.
-  Cursor look = start(first), load = look, at = look;
+  Cursor look = axis_start(cum, seqs, units, first), load = look, at = look;
   int looked = first, loaded = first, q_loads = 0;
   const auto look_and_store = [&]() {
     if (looked >= last) return;
     if (tid < kTile) row_at[(looked & 1) * kTile + tid] = lookup(look, tid);
-    next(look);
+    axis_next(cum, seqs, units, look);
     ++looked;
   };
   const auto load_one = [&]() {
@@ -309,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
       const bool with_q = loaded == first || load.tile == 0;
       if (with_q) ++q_loads;
       issue(load, (loaded - first) % kStages, loaded & 1, q_loads % kStages, with_q);
-      next(load);
+      axis_next(cum, seqs, units, load);
       ++loaded;
     }
     copy_commit();
@@ -505,39 +551,28 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = wr * 16 + quad_row + 8 * i;
-          const Row x = row_of<kShared>(a, at.b, kv_head, row0 + r);
-          if (!x.real) continue;
-          if (whole) {
-            const float inv = lim[i] > 0 ? 1.0f / l[i] : 0.0f;
-            T* dst = (T*)a.out + (((long long)x.b * a.tokens + x.t) * a.q_heads + x.head) * a.head_dim;
-#pragma unroll
-            for (int n = 0; n < kDt; ++n) {
-              const int c = n * 8 + (lane & 3) * 2;
-              if (c < a.head_dim)
-                *reinterpret_cast<unsigned*>(dst + c) =
-                    lim[i] > 0 ? pack2(o[n][2 * i] * inv, o[n][2 * i + 1] * inv, T{}) : 0u;
-            }
-          } else {
-            float* dst = a.part + (slot * kRows + r) * a.head_dim;
-#pragma unroll
-            for (int n = 0; n < kDt; ++n) {
-              const int c = n * 8 + (lane & 3) * 2;
-              if (c < a.head_dim) *reinterpret_cast<float2*>(dst + c) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-            }
-            if ((lane & 3) == 0) a.ml[slot * kRows + r] = make_float2(m[i], l[i]);
-          }
+          write_row<T, DT>(a, row_of<kShared>(a, at.b, kv_head, row0 + r), whole, lim[i] > 0, slot * kRows + r, lane, o, i,
+                           m[i], l[i]);
         }
       }
     }
-    next(at);
+    axis_next(cum, seqs, units, at);
     if (looking) {
       if (tid < kTile) row_at[(looked & 1) * kTile + tid] = next_row;
-      next(look);
+      axis_next(cum, seqs, units, look);
       ++looked;
     }
   }
   copy_wait<0>();
 }
+
+}  // namespace
+}  // namespace ckb
+
+#include "attention_stream.cuh"
+
+namespace ckb {
+namespace {
 
 // Joins the pieces of each output row: a warp per row (b, t, head).
 struct JoinArgs {
@@ -678,8 +713,60 @@ cudaError_t start(const Args& a, int ctas, cudaStream_t stream) {
   return launch_pdl(attend_tiles<T, DT, WR, kShared>, dim3(ctas), dim3(kThreads), bytes, stream, a);
 }
 
+// The cache as a TMA reads it: [rows][kv_heads][head_dim], boxes of box_rows rows of one head's 64 columns.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+template <typename T>
+bool cache_map(const Args& a, const void* cache, int box_rows, CUtensorMap& map) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const cuuint64_t rows = (cuuint64_t)a.num_blocks * a.block_size;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.kv_heads, rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.head_dim * a.kv_heads * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      sizeof(T) == 2 && std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(&map, type, 3, const_cast<void*>(cache), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Whether boxes of whole pages, or of 64 rows of a page, make up a tile (see attention_stream.cuh).
+bool boxes_fit(const Args& a) {
+  return a.block_size % 8 == 0 && (kTile % a.block_size == 0 || a.block_size % kTile == 0) && a.num_blocks > 0 &&
+         a.num_blocks * a.block_size < INT_MAX;
+}
+
+template <typename T, int DT, int WR>
+cudaError_t start_stream(const Args& a, int ctas, const CUtensorMap& keys, const CUtensorMap& values, cudaStream_t stream) {
+  const int bytes = Ring<DT, WR>::bytes(a.batch);
+  const cudaError_t err =
+      cudaFuncSetAttribute(attend_stream<T, DT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(attend_stream<T, DT, WR>, dim3(ctas), dim3(32 * (kConsumers + 1)), bytes, stream, a, keys, values);
+}
+
 template <typename T, int DT>
 cudaError_t start_own(const Args& a, int warps, int ctas, cudaStream_t stream) {
+  CUtensorMap keys, values;
+  const int box_rows = a.block_size < kTile ? a.block_size : kTile;
+  if (boxes_fit(a) && cache_map<T>(a, a.key, box_rows, keys) && cache_map<T>(a, a.value, box_rows, values)) {
+    if (warps == 1) return start_stream<T, DT, 1>(a, ctas, keys, values, stream);
+    if (warps == 2) return start_stream<T, DT, 2>(a, ctas, keys, values, stream);
+    return start_stream<T, DT, 4>(a, ctas, keys, values, stream);
+  }
   if (warps == 1) return start<T, DT, 1, false>(a, ctas, stream);
   if (warps == 2) return start<T, DT, 2, false>(a, ctas, stream);
   return start<T, DT, 4, false>(a, ctas, stream);
@@ -769,4 +856,17 @@ CKB_EXPORT int ckb_attention_paged_launch(const void* q, const void* key_cache, 
   if (dtype == kBF16) return start_all<__nv_bfloat16>(a, z, w, stream);
   if (dtype == kF16) return start_all<__half>(a, z, w, stream);
   return -1;
+}
+
+// Status of the bounded waits since the last reset: 0, or 1 when a wait gave up (that launch's output is void).
+CKB_EXPORT int ckb_attention_status(int reset) {
+  unsigned int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(v));
+  if (e != cudaSuccess) return -(int)e;
+  if (reset && v != 0u) {
+    const unsigned int zero = 0u;
+    e = cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero));
+    if (e != cudaSuccess) return -(int)e;
+  }
+  return (int)v;
 }

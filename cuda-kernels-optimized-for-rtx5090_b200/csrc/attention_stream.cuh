@@ -1,0 +1,365 @@
+// Own tokens, with the cache's tiles brought by TMA (included by attention.cu, whose parts it uses).
+//
+// The same axis of tiles, pieces and joins as attend_tiles. What bounds this work is the cache's bytes, and what kept
+// attend_tiles from their rate was instructions: 128 threads spent two thirds of them on addresses and copies of 16 bytes,
+// and a block barrier per tile held the warps in step (48 sequences of up to 16001 tokens: 389 us, 4.1 TB/s). Here one
+// warp looks the pages up and issues a TMA box for each page and 64 columns, and the four others only multiply; each
+// goes on as soon as a tile has arrived (mbarriers), whatever the others do.
+//
+// A box is one page (or a 64-row part of one), so the block size has to divide 64 or be a multiple of it, in steps of 8
+// rows (the swizzle's period); other block sizes, and caches of 2^31 rows, go through attend_tiles.
+#pragma once
+
+#include <cuda.h>
+
+namespace ckb {
+namespace {
+
+__device__ unsigned int g_attention_status = 0u;
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Arrives on bar when this thread's earlier cp.async copies are done (one of the expected arrivals).
+__device__ __forceinline__ void mbar_arrive_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load3(unsigned dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// Waits for a phase unless an earlier wait of this thread ran out: then the kernel runs on to its end without waiting
+// (its results are void, the status says so).
+__device__ __forceinline__ void wait_or_give_up(uint64_t* bar, unsigned parity, bool& dead) {
+  if (dead) return;
+  if (!mbar_wait(bar, parity)) {
+    dead = true;
+    atomicOr(&g_attention_status, CKB_STATUS_TIMEOUT);
+  }
+}
+__device__ __forceinline__ void sync_warps(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// A tile in shared memory: DT / 64 halves of [64 rows][128 bytes], 16-byte chunks exchanged within a row as the TMA's
+// 128-byte swizzle does. Byte offset of chunk c (of the whole row) of row r.
+__device__ __forceinline__ unsigned at_box(int r, int c) {
+  return (c >> 3) * (kTile * 128) + r * 128 + (((c ^ r) & 7) << 4);
+}
+
+constexpr int kConsumers = 4;  // warps that multiply; one more loads
+
+template <int DT, int WR>
+struct Ring {
+  static constexpr int kRows = 16 * WR;
+  static constexpr int kKeyWarps = 4 / WR;
+  static constexpr int kKeys = kTile / kKeyWarps;
+  static constexpr int kStages = WR == 1 && DT <= 128 ? 3 : 2;
+  static constexpr int kTileBytes = kTile * DT * 2;
+  static constexpr int kQBytes = kRows * DT * 2;
+  static constexpr int kOffQ = kStages * 2 * kTileBytes;
+  static constexpr int kOffMl = kOffQ + kStages * kQBytes;
+  static constexpr int kOffBars = kOffMl + kKeyWarps * kRows * 8;
+  static constexpr int kOffCum = kOffBars + 2 * kStages * 8;
+  static int bytes(int batch) { return kOffCum + (2 * batch + 1) * 4 + 1024; }  // 1024: the tiles' alignment
+};
+
+template <typename T, int DT, int WR>
+__global__ void __launch_bounds__(32 * (kConsumers + 1))
+    attend_stream(const Args a, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
+  using S = Ring<DT, WR>;
+  constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages, kHalves = DT / 64;
+  constexpr int kAll = 32 * (kConsumers + 1);
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float2* ml_sh = reinterpret_cast<float2*>(smem + S::kOffMl);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
+  uint64_t* empty = full + kStages;
+  int* cum = reinterpret_cast<int*>(smem + S::kOffCum);
+  int* lens = cum + a.batch + 1;
+  const unsigned smem_at = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 33);  // every lane of the loading warp, and its announcement of the bytes
+      mbar_init(&empty[i], kConsumers);
+    }
+    mbar_fence_init();
+  }
+  pdl_wait();
+  pdl_trigger();
+  const int units = a.kv_heads * a.row_tiles;
+  own_axis<kAll>(a, units, cum, lens, reinterpret_cast<int*>(ml_sh));  // its barriers order the mbarriers' set-up too
+  const int all = cum[a.batch];
+  const int run = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= a.batch; b += kAll) a.plan[b] = cum[b];
+    if (tid == 0) a.plan[a.batch + 1] = run;
+  }
+  const int first = (int)min((long long)blockIdx.x * run, (long long)all);
+  const int last = min(first + run, all);
+  if (first >= last) return;
+  Cursor at = axis_start(cum, a.batch, units, first);
+  bool dead = false;
+
+  if (warp == kConsumers) {
+    // Pages of a tile: box_rows rows each.
+    const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kTile / box_rows;
+    const int box_bytes = box_rows * 128;
+    const auto page_of = [&](const Cursor& c) -> int {  // lane p: the cache row where page p of the tile begins
+      const int pos = a.prefix + c.tile * kTile + lane * box_rows;
+      if (lane >= pages || pos >= lens[c.b]) return -1;
+      const int page = pos / a.block_size;
+      const long long block = __ldg(a.tables + (long long)c.b * a.table_width + page);
+      if (block < 0 || block >= a.num_blocks) return (int)(a.num_blocks * a.block_size);  // outside the map: zeros
+      return (int)(block * a.block_size + (pos - page * a.block_size));
+    };
+    int q_loads = 0;
+    int row_now = page_of(at);
+    for (int w = first; w < last; ++w) {
+      const int stage = (w - first) % kStages;
+      const int kv_head = at.unit / a.row_tiles;
+      Cursor ahead = at;
+      axis_next(cum, a.batch, units, ahead);
+      const int row_next = w + 1 < last ? page_of(ahead) : -1;  // behind this tile's copies
+      wait_or_give_up(&empty[stage], (((w - first) / kStages) & 1) ^ 1, dead);
+      if (dead) return;
+      const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], there * box_bytes * kHalves * 2);
+      for (int i = lane; __any_sync(0xffffffffu, i < pages * kHalves * 2); i += 32) {
+        const int page = i % pages, half = i / pages % kHalves, is_v = i / (pages * kHalves);
+        const int row = __shfl_sync(0xffffffffu, row_now, page);
+        if (i < pages * kHalves * 2 && row >= 0)
+          tma_load3(smem_at + (stage * 2 + is_v) * S::kTileBytes + half * (kTile * 128) + page * box_bytes,
+                    is_v ? &value_map : &key_map, half * 64, kv_head, row, &full[stage]);
+      }
+      if (w == first || at.tile == 0) {  // a piece begins: its queries come with its first tile
+        const int row0 = (at.unit - kv_head * a.row_tiles) * kRows;
+        for (int i = lane; i < kRows * (DT / 8); i += 32) {
+          const int r = i / (DT / 8), chunk = i % (DT / 8);
+          const Row x = row_of<false>(a, at.b, kv_head, row0 + r);
+          const bool fill = x.real && chunk * 8 < a.head_dim;
+          const long long off = fill ? x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head + chunk * 8 : 0;
+          copy16(smem_at + S::kOffQ + (q_loads % kStages) * S::kQBytes + at_chunk<DT>(r, chunk), (const T*)a.q + off, fill);
+        }
+        ++q_loads;
+        mbar_arrive_copies(&full[stage]);
+      } else {
+        mbar_arrive(&full[stage]);
+      }
+      at = ahead;
+      row_now = row_next;
+    }
+    copy_commit();
+    copy_wait<0>();
+    return;
+  }
+
+  const int wr = warp % WR, wk = warp / WR, quad_row = lane >> 2;
+  constexpr int kNt = kKeys / 8, kDt = DT / 8;
+  float o[kDt][4], m[2], l[2];
+  int len = 0, min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
+  for (int w = first; w < last; ++w) {
+    const int stage = (w - first) % kStages;
+    const int kv_head = at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
+    if (w == first || at.tile == 0) {  // a new piece
+      ++q_now;
+      piece_begin = at.tile;
+      len = lens[at.b];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int in = row0 + wr * 16 + quad_row + 8 * i;
+        lim[i] = in < a.rows ? max(0, len - a.tokens + in / a.group + 1) : INT_MAX;  // padding: any finite result
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+      }
+      min_limit = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));
+#pragma unroll
+      for (int n = 0; n < kDt; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+    }
+    wait_or_give_up(&full[stage], ((w - first) / kStages) & 1, dead);
+
+    const unsigned k_at = smem_at + stage * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
+    const unsigned q_at = smem_at + S::kOffQ + ((q_now - 1) % kStages) * S::kQBytes;
+    const int pos0 = a.prefix + at.tile * kTile + wk * kKeys;
+    float s[kNt][4];
+#pragma unroll
+    for (int n = 0; n < kNt; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DT / 16; ++k) {
+      unsigned qa[4];
+      ldsm4(qa, q_at + at_chunk<DT>(wr * 16 + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+      for (int n = 0; n < kNt; n += 2) {
+        unsigned kb[4];
+        ldsm4(kb, k_at + at_box(wk * kKeys + n * 8 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
+        mma(s[n], qa, kb[0], kb[1], T{});
+        mma(s[n + 1], qa, kb[2], kb[3], T{});
+      }
+    }
+    const bool masked = pos0 + kKeys > min_limit;
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (pos0 + n * 8 + (lane & 3) * 2 + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
+    }
+    float top[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = m[i];
+#pragma unroll
+      for (int n = 0; n < kNt; ++n) top[i] = fmaxf(top[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]) * a.scale_log2);
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {  // a new maximum: rarer and rarer along the tiles
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float scale = exp2_fast(m[i] - (top[i] == -INFINITY ? 0.0f : top[i]));
+        m[i] = top[i];
+        l[i] *= scale;
+#pragma unroll
+        for (int n = 0; n < kDt; ++n) {
+          o[n][2 * i] *= scale;
+          o[n][2 * i + 1] *= scale;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float ref = m[i] == -INFINITY ? 0.0f : m[i];  // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = exp2_fast(fmaf(s[n][2 * i + e], a.scale_log2, -ref));
+          s[n][2 * i + e] = p;
+          sum += p;
+        }
+      l[i] += sum;
+    }
+    if (pos0 + kKeys > len) {  // what lies behind the sequence in its last page is anything: 0 * v must be 0
+      for (int i = lane; i < kKeys * (DT / 8); i += 32) {
+        const int r = i / (DT / 8);
+        if (pos0 + r >= len)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + at_box(wk * kKeys + r, i % (DT / 8))), "r"(0u)
+                       : "memory");
+      }
+      __syncwarp();
+      fence_proxy_async();  // before the ring's next copy into these bytes
+    }
+    if (masked && a.tokens > 1 && not_finite_box<T, DT, kKeys>(v_at, wk * kKeys, lane)) {
+      // A value that some row must not see is not finite: 0 * v would carry it over. One position after the other.
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+        for (int j = 0; j < 8; ++j) {
+          const int key = n * 8 + j, from = (lane & ~3) | (j >> 1);
+          const float p0 = round_through<T>(__shfl_sync(0xffffffffu, j & 1 ? s[n][1] : s[n][0], from));
+          const float p1 = round_through<T>(__shfl_sync(0xffffffffu, j & 1 ? s[n][3] : s[n][2], from));
+          const bool see0 = pos0 + key < lim[0], see1 = pos0 + key < lim[1];
+#pragma unroll
+          for (int c = 0; c < kDt; ++c) {
+            const float2 v = load2(v_at + at_box(wk * kKeys + key, c) + (lane & 3) * 4, T{});
+            if (see0) {
+              o[c][0] = fmaf(p0, v.x, o[c][0]);
+              o[c][1] = fmaf(p0, v.y, o[c][1]);
+            }
+            if (see1) {
+              o[c][2] = fmaf(p1, v.x, o[c][2]);
+              o[c][3] = fmaf(p1, v.y, o[c][3]);
+            }
+          }
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k) {
+        unsigned pa[4];
+        pa[0] = pack2(s[2 * k][0], s[2 * k][1], T{});
+        pa[1] = pack2(s[2 * k][2], s[2 * k][3], T{});
+        pa[2] = pack2(s[2 * k + 1][0], s[2 * k + 1][1], T{});
+        pa[3] = pack2(s[2 * k + 1][2], s[2 * k + 1][3], T{});
+#pragma unroll
+        for (int n = 0; n < kDt; n += 2) {
+          unsigned vb[4];
+          ldsm4_trans(vb, v_at + at_box(wk * kKeys + k * 16 + (lane & 15), n + (lane >> 4)));
+          mma(o[n], pa, vb[0], vb[1], T{});
+          mma(o[n + 1], pa, vb[2], vb[3], T{});
+        }
+      }
+    }
+
+    if (at.tile + 1 == at.tiles || w + 1 == last) {  // the end of a piece
+      const bool whole = a.prefix == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
+      const long long slot = (long long)at.b * units + at.unit + blockIdx.x;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      if (S::kKeyWarps > 1) {  // join the warps that shared the positions, in the tile's own stage
+        if ((lane & 3) == 0) {
+          ml_sh[wk * kRows + wr * 16 + quad_row] = make_float2(m[0], l[0]);
+          ml_sh[wk * kRows + wr * 16 + quad_row + 8] = make_float2(m[1], l[1]);
+        }
+        sync_warps(1, 32 * kConsumers);  // and nobody reads the tile any more
+        float* sum_o = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);
+        float weight[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = wr * 16 + quad_row + 8 * i;
+          const float mine = m[i];
+          float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) most = fmaxf(most, ml_sh[k * kRows + r].x);
+          const float ref = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) sum += ml_sh[k * kRows + r].y * exp2_fast(ml_sh[k * kRows + r].x - ref);
+          weight[i] = exp2_fast(mine - ref);
+          m[i] = most;
+          l[i] = sum;
+        }
+        for (int k = 0; k < S::kKeyWarps; ++k) {
+          if (wk == k) {
+#pragma unroll
+            for (int n = 0; n < kDt; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float2* dst = reinterpret_cast<float2*>(sum_o + (wr * 16 + quad_row + 8 * i) * DT + n * 8 + (lane & 3) * 2);
+                float2 v = make_float2(o[n][2 * i] * weight[i], o[n][2 * i + 1] * weight[i]);
+                if (k > 0) {
+                  const float2 u = *dst;
+                  v.x += u.x;
+                  v.y += u.y;
+                }
+                *dst = v;
+                o[n][2 * i] = v.x;
+                o[n][2 * i + 1] = v.y;
+              }
+          }
+          sync_warps(1, 32 * kConsumers);
+        }
+        fence_proxy_async();
+      }
+      if (wk == S::kKeyWarps - 1) {  // the last to add holds the sums
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          write_row<T, DT>(a, row_of<false>(a, at.b, kv_head, row0 + wr * 16 + quad_row + 8 * i), whole, lim[i] > 0,
+                           slot * kRows + wr * 16 + quad_row + 8 * i, lane, o, i, m[i], l[i]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+    axis_next(cum, a.batch, units, at);
+  }
+}
+
+}  // namespace
+}  // namespace ckb

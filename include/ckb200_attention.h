@@ -22,13 +22,17 @@ long long ckb_attention_workspace(long long batch, int tokens, int q_heads, int 
  * + t + 1; out [batch, tokens, q_heads, head_dim] (contiguous) = softmax(scale * q . k) v over them, zeros where there
  * are none. q head h reads kv head h / (q_heads / kv_heads). shared_prefix: a multiple of block_size; the first
  * shared_prefix tokens are the same blocks for the whole batch and are read through row 0 of tables, once for all.
- * head_dim a multiple of 8, at most 256; batch at most 8192. work: the workspace (16-byte aligned, contents do not
+ * head_dim a multiple of 8, at most 256; batch at most 4096. work: the workspace (16-byte aligned, contents do not
  * matter before and after). No counterpart in the reference. */
 int ckb_attention_paged_launch(const void* q, const void* key_cache, const void* value_cache, const void* tables,
                                const void* lens, void* out, void* work, long long work_bytes,
                                const long long* q_strides, long long batch, int tokens, int q_heads, int kv_heads,
                                int head_dim, long long num_blocks, int block_size, long long table_width,
                                long long shared_prefix, float scale, int dtype, cudaStream_t stream);
+
+/* Bounded-wait status of the kernels since the last reset: 0 fine, 1 a wait for a copy gave up after 2 s (that launch's
+ * output is void), negative a cudaError_t from reading it. Synchronises the device. */
+int ckb_attention_status(int reset);
 
 #ifdef __cplusplus
 }

@@ -82,6 +82,10 @@ OWN = [  # dtype, T, Hq, Hkv, D, block size, lengths
     (BF, 1, 8, 2, 128, 16, [4000]),  # a row cut into many pieces
     (BF, 1, 2, 1, 64, 16, [17] * 200),  # many sequences of one tile
     (HF, 3, 8, 4, 128, 16, list(range(0, 190, 3))),
+    (BF, 1, 8, 2, 128, 8, [100, 9, 64]),
+    (HF, 2, 8, 2, 64, 256, [300, 65, 513]),
+    (BF, 1, 8, 2, 136, 24, [100, 9]),
+    (BF, 1, 2, 2, 64, 16, [i % 130 for i in range(600)]),  # more sequences than threads
 ]
 
 
@@ -229,6 +233,12 @@ def test_streams_repeats_and_graphs_that_share_a_pool():
     graphs[0].replay()
     torch.cuda.synchronize()
     assert bits_equal(outs[0], attention.paged_attention(*a, shared_prefix=64))
+
+
+def test_no_wait_has_given_up():
+    from ckb200 import _native
+
+    assert _native.load("attention").ckb_attention_status(0) == 0
 
 
 def test_a_drafted_decoding_step():

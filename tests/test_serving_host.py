@@ -123,7 +123,7 @@ def test_attention_abi_refusals():
     sizes = (2, 3, 4, 2, 64, 16, 4, 0)
     need = lib.ckb_attention_workspace(*sizes)
     assert need > 0
-    for i, v in ((0, 0), (0, 8193), (1, 0), (2, 3), (2, 0), (3, 0), (4, 0), (4, 12), (4, 264), (5, 0), (6, 0), (6, 1 << 40),
+    for i, v in ((0, 0), (0, 4097), (1, 0), (2, 3), (2, 0), (3, 0), (4, 0), (4, 12), (4, 264), (5, 0), (6, 0), (6, 1 << 40),
                  (7, 8), (7, -16), (7, 80)):
         assert lib.ckb_attention_workspace(*sizes[:i], v, *sizes[i + 1:]) == -1, (i, v)
     assert lib.ckb_attention_workspace(1, 1, 32, 8, 128, 16, 8192, 0) < 64 << 20  # a long table costs nothing
@@ -133,7 +133,7 @@ def test_attention_abi_refusals():
     assert fn(*good[:9], 0, *good[10:]) == 0
     odd = (ctypes.c_longlong * 3)(768, 256, 60)
     for i, v in ((0, None), (0, 8), (1, None), (1, 24), (2, 24), (3, None), (4, None), (5, None), (5, 8), (6, None), (6, 8),
-                 (7, need - 1), (8, None), (8, odd), (9, 8193), (10, 0), (11, 3), (13, 60), (14, -1), (15, 0), (16, 0),
+                 (7, need - 1), (8, None), (8, odd), (9, 4097), (10, 0), (11, 3), (13, 60), (14, -1), (15, 0), (16, 0),
                  (17, 8), (18, 0.0), (18, -1.0), (18, float("nan")), (18, float("inf")), (19, 0), (19, 3)):
         assert fn(*good[:i], v, *good[i + 1:]) == -1, (i, v)
 
