@@ -160,10 +160,12 @@ __device__ __forceinline__ long long length_of(const Args& a, int b) {
   const long long most = (long long)a.table_width * a.block_size, n = __ldg(a.lens + b);
   return n < 0 ? 0 : n < most ? n : most;
 }
-// The positions that token t of sequence b sees: those below this (none if it is not positive).
-__device__ __forceinline__ int limit_of(const Args& a, int b, int t) {
-  return (int)length_of(a, b) - a.tokens + t + 1;
+// Where a sequence's own positions begin: behind the prefix, or, for one that does not see all of it, at 0: such a sequence
+// (shorter than the prefix, or none) takes no part in the shared work, whose rows all see every position.
+__device__ __forceinline__ int own_begin(int prefix, int tokens, int len) {
+  return len - tokens + 1 >= prefix ? prefix : 0;
 }
+
 // A place on the axis of tiles.
 struct Cursor {
   int b, unit, tile, tiles;  // sequence (0 in shared work), unit within it, tile within the unit, the unit's tiles
@@ -181,7 +183,7 @@ __device__ __forceinline__ void own_axis(const Args& a, int units, int* cum, int
     if (b < a.batch) {
       const int len = (int)length_of(a, b);
       lens[b] = len;
-      mine = len > a.prefix ? (len - a.prefix + kTile - 1) / kTile * units : 0;
+      mine = (len - own_begin(a.prefix, a.tokens, len) + kTile - 1) / kTile * units;
     }
     int upto = mine;
 #pragma unroll
@@ -309,8 +311,8 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
 
   // The cache row of position (tile, lane of the tile), or -1.
   const auto lookup = [&](const Cursor& c, int i) -> long long {
-    const int pos = (kShared ? 0 : a.prefix) + c.tile * kTile + i;
     const int end = kShared ? a.prefix : cum[a.batch + 1 + c.b];
+    const int pos = (kShared ? 0 : own_begin(a.prefix, a.tokens, end)) + c.tile * kTile + i;
     if (pos >= end) return -1;
     const int page = pos / a.block_size;
     const long long block = __ldg(a.tables + (kShared ? 0LL : (long long)c.b * a.table_width) + page);
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   constexpr int kNt = kKeys / 8;   // score tiles of 8 positions
   constexpr int kDt = DT / 8;      // output tiles of 8 columns
   float o[kDt][4], m[2], l[2];
-  int min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
+  int min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0, begin = 0;
   const int quad_row = lane >> 2;
   for (int w = first; w < last; ++w) {
     copy_wait<kStages - 2>();
@@ -384,10 +386,11 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
     if (w == first || at.tile == 0) {  // a new piece
       ++q_now;
       piece_begin = at.tile;
+      begin = kShared ? 0 : own_begin(a.prefix, a.tokens, cum[a.batch + 1 + at.b]);
       if (tid < kRows) {
         const Row x = row_of<kShared>(a, at.b, kv_head, row0 + tid);
-        const int n = x.real ? max(0, limit_of(a, x.b, x.t)) : INT_MAX;  // a row of padding: any finite result
-        limits[tid] = kShared ? min(n, a.prefix) : n;
+        // A row of padding: any finite result.
+        limits[tid] = kShared ? a.prefix : x.real ? max(0, cum[a.batch + 1 + at.b] - a.tokens + x.t + 1) : INT_MAX;
       }
       __syncthreads();
       min_limit = INT_MAX;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
 
     const unsigned k_at = smem_at + ((w - first) % kStages) * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
     const unsigned q_at = smem_at + S::kOffQ + (q_now % kStages) * S::kQBytes;
-    const int pos0 = (kShared ? 0 : a.prefix) + at.tile * kTile + wk * kKeys;
+    const int pos0 = begin + at.tile * kTile + wk * kKeys;
     float s[kNt][4];
 #pragma unroll
     for (int n = 0; n < kNt; ++n)
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
     }
 
     if (at.tile + 1 == at.tiles || w + 1 == last) {  // the end of a piece
-      const bool whole = !kShared && a.prefix == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
+      const bool whole = !kShared && begin == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
       const long long slot = (long long)at.b * units + at.unit + blockIdx.x;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -570,6 +573,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
 }  // namespace ckb
 
 #include "attention_stream.cuh"
+#include "attention_prefix.cuh"
 
 namespace ckb {
 namespace {
@@ -583,8 +587,10 @@ struct JoinArgs {
   const int* plan;
   int batch, tokens, q_heads, kv_heads, group, head_dim, prefix, rows, table_positions;
   int own_rows, own_row_tiles;        // rows of an own slot, row tiles of an own unit
-  int shared_rows, shared_row_tiles;  // the same of the shared work (0: none)
+  int shared_rows, shared_unit_rows;  // rows of a slot and of a unit of the shared work
+  int shared_row_tiles;               // 0: none
   int shared_tiles, shared_run;       // tiles of a shared unit, tiles of a run
+  int shared_slots, shared_split;     // slots of a piece; whether they are parts of the positions, not of the rows
 };
 
 template <typename T>
@@ -600,25 +606,31 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
   // Own pieces: slots own_slot, own_slot + 1, ...; shared ones the same.
   const int units = a.kv_heads * a.own_row_tiles, unit = kv_head * a.own_row_tiles + in / a.own_rows;
   const int begin = a.plan[b], tiles = (a.plan[b + 1] - begin) / units, run = a.plan[a.batch + 1];
+  const long long n = a.lens[b];
+  const int len = (int)(n < 0 ? 0 : n < a.table_positions ? n : a.table_positions);
+  const bool sharing = a.shared_row_tiles > 0 && own_begin(a.prefix, a.tokens, len) > 0;
   int own = 0;
-  long long own_slot = 0;
+  long long own_at = 0;  // workspace row of the first own piece
   if (tiles > 0) {
     const int w0 = begin + unit * tiles, c0 = w0 / run;
     own = (w0 + tiles - 1) / run - c0 + 1;
-    own_slot = (long long)b * units + unit + c0;
-    if (own == 1 && a.prefix == 0) return;  // written out by its CTA
+    own_at = ((long long)b * units + unit + c0) * a.own_rows + in % a.own_rows;
+    if (own == 1 && !sharing) return;  // written out by its CTA
   }
-  int shared = 0;
-  long long shared_slot = 0;
-  const int all_row = b * a.rows + in;
-  if (a.shared_row_tiles > 0) {
-    const int u = kv_head * a.shared_row_tiles + all_row / a.shared_rows, w0 = u * a.shared_tiles, c0 = w0 / a.shared_run;
+  int shared = 0, shared_step = 0;
+  long long shared_at = 0;
+  if (sharing) {
+    const int all_row = b * a.rows + in, in_unit = all_row % a.shared_unit_rows;
+    const int u = kv_head * a.shared_row_tiles + all_row / a.shared_unit_rows, w0 = u * a.shared_tiles, c0 = w0 / a.shared_run;
     shared = (w0 + a.shared_tiles - 1) / a.shared_run - c0 + 1;
-    shared_slot = u + c0;
+    shared_step = a.shared_slots * a.shared_rows;
+    shared_at = (u + (long long)c0) * shared_step + in_unit;  // slots of the unit's row tiles lie one after the other
+    if (a.shared_split) {
+      shared *= a.shared_slots;
+      shared_step = a.shared_rows;
+    }
   }
-  const long long own_at = own_slot * a.own_rows + in % a.own_rows;
-  const long long shared_at = a.shared_row_tiles > 0 ? shared_slot * a.shared_rows + all_row % a.shared_rows : 0;
-  const auto at = [&](int i) { return i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * a.shared_rows; };
+  const auto at = [&](int i) { return i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * shared_step; };
   const int pieces = own + shared;
   float top = -INFINITY;
   for (int i = lane; i < pieces; i += 32) top = fmaxf(top, (i < own ? a.own_ml : a.shared_ml)[at(i)].x);
@@ -630,8 +642,7 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
     sum += v.y * exp2_fast(v.x - ref);
   }
   sum = warp_sum(sum);
-  const long long n = a.lens[b], most = n < 0 ? 0 : n < a.table_positions ? n : a.table_positions;
-  const bool some = most - a.tokens + t + 1 > 0;
+  const bool some = len - a.tokens + t + 1 > 0;
   T* out = (T*)a.out + row * a.head_dim;
   for (int c = lane * 4; c < a.head_dim; c += 128) {
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -657,8 +668,9 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
 // ---------------------------------------------------------------------------------------------------------------
 struct Sizes {
   int rows, own_warps, own_rows, own_row_tiles, own_ctas;
-  int shared_row_tiles, shared_tiles, shared_ctas, shared_run;
-  long long own_slots, shared_slots, off_plan, off_own_ml, off_own, off_shared_ml, off_shared, bytes;
+  // The shared work on the tensor cores of the fifth generation (0), or by attend_tiles (1).
+  struct { int unit_rows, row_tiles, tiles, ctas, run, rows, slots; } shared[2];
+  long long own_slots, off_plan, off_own_ml, off_own, off_shared_ml, off_shared, bytes;
 };
 
 // CTAs of attend_tiles on an SM, by shared memory: 2 or 3 stages of 16, 32 or 64 KB for head_dim up to 64, 128 and 256.
@@ -684,22 +696,29 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
   const int most = device_sm_count() * per_sm(head_dim);
   z.own_ctas = most;
   z.own_slots = batch * kv_heads * z.own_row_tiles + z.own_ctas;
-  if (prefix > 0) {
-    z.shared_row_tiles = (int)((rows * batch + 63) / 64);
-    z.shared_tiles = (int)((prefix + kTile - 1) / kTile);
-    const long long all = (long long)z.shared_tiles * kv_heads * z.shared_row_tiles;
+  long long shared_rows = 0;  // of the workspace
+  for (int i = 0; i < 2 && prefix > 0; ++i) {
+    auto& h = z.shared[i];
+    h.rows = i == 0 ? kGroupRows : 64;
+    h.unit_rows = i == 0 && rows * batch > kGroupRows ? 2 * kGroupRows : h.rows;
+    h.slots = i == 0 ? 2 : 1;
+    h.row_tiles = (int)((rows * batch + h.unit_rows - 1) / h.unit_rows);
+    const int tile = i == 0 ? kPrefixTile : kTile, at_once = i == 0 ? device_sm_count() : most;
+    h.tiles = (int)((prefix + tile - 1) / tile);
+    const long long all = (long long)h.tiles * kv_heads * h.row_tiles;
     if (all > INT_MAX / 2) return false;
-    z.shared_ctas = (int)(all < most ? all : most);
-    z.shared_run = (int)((all + z.shared_ctas - 1) / z.shared_ctas);
-    z.shared_slots = (long long)kv_heads * z.shared_row_tiles + z.shared_ctas;
+    h.run = (int)((all + at_once - 1) / at_once);
+    h.ctas = (int)((all + h.run - 1) / h.run);
+    const long long need = ((long long)kv_heads * h.row_tiles + h.ctas) * h.slots * h.rows;
+    if (need > shared_rows) shared_rows = need;
   }
   const auto up = [](long long n) { return (n + 255) / 256 * 256; };
   z.off_plan = 0;
   z.off_own_ml = up((batch + 2) * 4);
   z.off_own = z.off_own_ml + up(z.own_slots * z.own_rows * 8);
   z.off_shared_ml = z.off_own + up(z.own_slots * z.own_rows * head_dim * 4);
-  z.off_shared = z.off_shared_ml + up(z.shared_slots * 64 * 8);
-  z.bytes = z.off_shared + up(z.shared_slots * 64 * head_dim * 4);
+  z.off_shared = z.off_shared_ml + up(shared_rows * 8);
+  z.bytes = z.off_shared + up(shared_rows * head_dim * 4);
   return true;
 }
 
@@ -758,44 +777,66 @@ cudaError_t start_stream(const Args& a, int ctas, const CUtensorMap& keys, const
   return launch_pdl(attend_stream<T, DT, WR>, dim3(ctas), dim3(32 * (kConsumers + 1)), bytes, stream, a, keys, values);
 }
 
-template <typename T, int DT>
-cudaError_t start_own(const Args& a, int warps, int ctas, cudaStream_t stream) {
+struct Maps {
+  bool fit;
   CUtensorMap keys, values;
-  const int box_rows = a.block_size < kTile ? a.block_size : kTile;
-  if (boxes_fit(a) && cache_map<T>(a, a.key, box_rows, keys) && cache_map<T>(a, a.value, box_rows, values)) {
-    if (warps == 1) return start_stream<T, DT, 1>(a, ctas, keys, values, stream);
-    if (warps == 2) return start_stream<T, DT, 2>(a, ctas, keys, values, stream);
-    return start_stream<T, DT, 4>(a, ctas, keys, values, stream);
+};
+
+template <typename T, int DT>
+cudaError_t start_own(const Args& a, int warps, int ctas, const Maps& maps, cudaStream_t stream) {
+  if (maps.fit) {
+    if (warps == 1) return start_stream<T, DT, 1>(a, ctas, maps.keys, maps.values, stream);
+    if (warps == 2) return start_stream<T, DT, 2>(a, ctas, maps.keys, maps.values, stream);
+    return start_stream<T, DT, 4>(a, ctas, maps.keys, maps.values, stream);
   }
   if (warps == 1) return start<T, DT, 1, false>(a, ctas, stream);
   if (warps == 2) return start<T, DT, 2, false>(a, ctas, stream);
   return start<T, DT, 4, false>(a, ctas, stream);
 }
 
+template <typename T, int DT>
+cudaError_t start_prefix(const Args& a, const Sizes& z, const Maps& maps, cudaStream_t stream) {
+  const auto& h = z.shared[0];
+  const int bytes = PrefixShape<DT>::kBytes;
+  const cudaError_t err = cudaFuncSetAttribute(attend_prefix<T, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) return err;
+  const PrefixArgs p{a, h.tiles, h.run, h.unit_rows};
+  return launch_pdl(attend_prefix<T, DT>, dim3(h.ctas), dim3(kPrefixThreads), bytes, stream, p, maps.keys, maps.values);
+}
+
 template <typename T>
 int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) {
   const int dt = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+  const int box_rows = a.block_size < kTile ? a.block_size : kTile;
+  Maps maps;
+  maps.fit = boxes_fit(a) && cache_map<T>(a, a.key, box_rows, maps.keys) && cache_map<T>(a, a.value, box_rows, maps.values);
+  // Two groups' O and S of 256 columns each do not fit TMEM: heads of more than 128 columns take attend_tiles.
+  const bool tensor = maps.fit && dt <= 128;
+  const auto& h = z.shared[tensor ? 0 : 1];
   cudaError_t err = cudaSuccess;
   Args s = a;
   a.row_tiles = z.own_row_tiles;
   a.part = reinterpret_cast<float*>(work + z.off_own);
   a.ml = reinterpret_cast<float2*>(work + z.off_own_ml);
-  s.row_tiles = z.shared_row_tiles;
+  s.row_tiles = h.row_tiles;
   s.part = reinterpret_cast<float*>(work + z.off_shared);
   s.ml = reinterpret_cast<float2*>(work + z.off_shared_ml);
   if (a.prefix > 0) {
-    err = dt == 64 ? start<T, 64, 4, true>(s, z.shared_ctas, stream)
-          : dt == 128 ? start<T, 128, 4, true>(s, z.shared_ctas, stream)
-                      : start<T, 256, 4, true>(s, z.shared_ctas, stream);
+    if (tensor)
+      err = dt == 64 ? start_prefix<T, 64>(s, z, maps, stream) : start_prefix<T, 128>(s, z, maps, stream);
+    else
+      err = dt == 64 ? start<T, 64, 4, true>(s, h.ctas, stream)
+            : dt == 128 ? start<T, 128, 4, true>(s, h.ctas, stream)
+                        : start<T, 256, 4, true>(s, h.ctas, stream);
   }
   if (err == cudaSuccess)
-    err = dt == 64 ? start_own<T, 64>(a, z.own_warps, z.own_ctas, stream)
-          : dt == 128 ? start_own<T, 128>(a, z.own_warps, z.own_ctas, stream)
-                      : start_own<T, 256>(a, z.own_warps, z.own_ctas, stream);
+    err = dt == 64 ? start_own<T, 64>(a, z.own_warps, z.own_ctas, maps, stream)
+          : dt == 128 ? start_own<T, 128>(a, z.own_warps, z.own_ctas, maps, stream)
+                      : start_own<T, 256>(a, z.own_warps, z.own_ctas, maps, stream);
   if (err == cudaSuccess) {
     const JoinArgs j{a.out, a.lens, a.part, s.part, a.ml, s.ml, a.plan, a.batch, a.tokens, a.q_heads, a.kv_heads, a.group,
-                     a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, 64,
-                     z.shared_row_tiles, z.shared_tiles, z.shared_run};
+                     a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, h.rows,
+                     h.unit_rows, h.row_tiles, h.tiles, h.run, h.slots, h.unit_rows == h.rows && h.slots > 1};
     const long long rows = (long long)a.batch * a.tokens * a.q_heads;
     err = launch_pdl(join_rows<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, j);
   }

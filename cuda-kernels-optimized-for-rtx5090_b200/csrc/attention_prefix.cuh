@@ -1,0 +1,372 @@
+// The shared prefix on the fifth-generation tensor cores (included by attention.cu, whose parts it uses).
+//
+// A unit is a kv head and 256 (or, where the batch has no more, 128) of the query rows that share it, those of all
+// sequences one after the other; its tiles are 128 positions of the prefix. Every row sees every position, so nothing is
+// masked but the last tile's overhang. For 128 rows and 128 positions a tile takes 2 x 2 x 128 x 128 x D operations: at
+// D = 128 about 1024 clocks of an SM's tensor cores, and 128 x 128 exponentials, 1024 clocks of its MUFUs, while its keys and
+// values take about 2800 clocks of an SM's share of HBM, shared by the two row tiles of a unit and, through L2, by the
+// other units of the head. So the products and the exponentials have to run at the same time, and do:
+//   warps 0-3, 4-7  a softmax group each, a thread a row: scores S from TMEM, running maximum, exp, the weights P back to
+//                   TMEM in 16 bits over S, the sum of the unrounded weights in fp32;
+//   warp 8          looks the pages up and loads keys and values by TMA (rings of two tiles each);
+//   warp 9          issues S_i = Q_i K^T and O_i += P_i V (P_i from TMEM) for the two groups in turn: while one group
+//                   works on its scores, the tensor cores work for the other.
+// The two groups have a row tile of 128 each of a 256-row unit, or every other tile of positions of a 128-row unit (then
+// they are two pieces). O_i stays in TMEM. It is scaled down only when a row's maximum has risen by more than 8 (powers of
+// 2) over the one in use; until then weights may reach 2^8, which fp32 sums and 16-bit weights hold as well as 1.
+#pragma once
+
+namespace ckb {
+namespace {
+
+constexpr int kPrefixTile = 128;  // positions of a tile
+constexpr int kGroupRows = 128;   // query rows of a softmax group
+constexpr int kPrefixThreads = 384;  // warps 10 and 11 only fill the third warpgroup, which hands its registers over
+constexpr float kSlack = 8.0f;    // by how much a maximum may fall behind
+
+// ---------------------------------------------------------------------------------------------------------------
+// tcgen05 and TMEM, against the PTX ISA for sm_100a.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(unsigned* at, unsigned columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(unsigned at, unsigned columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D (+)= A B, A and B in shared memory.
+__device__ __forceinline__ void tc_mma(unsigned d, uint64_t a, uint64_t b, unsigned kind, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kind), "r"((unsigned)add)
+      : "memory");
+}
+// The same with A in TMEM.
+__device__ __forceinline__ void tc_mma_tmem(unsigned d, unsigned a, uint64_t b, unsigned kind, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(kind), "r"((unsigned)add)
+      : "memory");
+}
+// 32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_load32(unsigned at, unsigned (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(unsigned at, const unsigned (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+// Waits for this thread's loads. The values pass through it, so that no use of them is moved before it.
+__device__ __forceinline__ void tmem_wait_load(unsigned (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                 "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
+                 "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
+                 "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand with the 128-byte swizzle: 8 rows of 128 bytes are 1024 bytes apart (stride); `lead` is the distance
+// of the next 64 columns of an operand whose rows run along the sum (values), unused for one whose columns do (queries, keys).
+__device__ __forceinline__ uint64_t operand(unsigned at, unsigned lead) {
+  return (uint64_t)((at >> 4) & 0x3fffu) | (uint64_t)((lead >> 4) & 0x3fffu) << 16 | (uint64_t)(1024u >> 4) << 32 | 1ull << 46 |
+         2ull << 61;
+}
+// Instruction descriptor: fp32 sums, A and B of T, 128 rows, `columns` columns, B's rows along the sum where `b_rows`.
+template <typename T>
+__device__ __forceinline__ unsigned mma_kind(int columns, bool b_rows) {
+  const unsigned type = std::is_same<T, __half>::value ? 0u : 1u;
+  return 1u << 4 | type << 7 | type << 10 | (b_rows ? 1u << 16 : 0u) | (unsigned)(columns >> 3) << 17 | (128u >> 4) << 24;
+}
+
+struct PrefixArgs {
+  Args a;
+  int tiles, run;  // tiles of a unit, tiles of a CTA's run
+  int unit_rows;   // 256: the groups have 128 rows each; 128: they have every other tile each
+};
+
+template <int DT>
+struct PrefixShape {
+  static constexpr int kTileBytes = kPrefixTile * DT * 2;
+  static constexpr int kOffK = 2 * kGroupRows * DT * 2;
+  static constexpr int kOffV = kOffK + 2 * kTileBytes;
+  static constexpr int kOffBars = kOffV + 2 * kTileBytes;
+  static constexpr int kBytes = kOffBars + 16 * 8 + 16 + 1024;
+  static constexpr int kHalf = kPrefixTile * 128;  // bytes of 64 columns of a tile
+};
+
+template <typename T, int DT>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    attend_prefix(const PrefixArgs p, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
+  using S = PrefixShape<DT>;
+  const Args& a = p.a;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const unsigned smem_at = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;  // by stage
+  uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12, *o_full = bars + 14;  // by group
+  unsigned* tmem_sh = reinterpret_cast<unsigned*>(bars + 16);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&q_full[i], kGroupRows);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kGroupRows);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_sh, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = *tmem_sh;  // columns: S_0 | S_1 (128 each, P_i over S_i), then O_0 | O_1
+  pdl_wait();
+  pdl_trigger();
+
+  const int units = a.kv_heads * a.row_tiles;
+  const bool alternate = p.unit_rows == kGroupRows;
+  const int first = blockIdx.x * p.run, last = min(first + p.run, units * p.tiles);
+  bool dead = false;
+  // 168 registers a thread at launch: 384 x 168 = 64512 >= 256 x 208 + 128 x 80.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8) {
+      const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kPrefixTile / box_rows;
+      const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
+        const int pos = tile * kPrefixTile + lane * box_rows;
+        const int outside = (int)(a.num_blocks * a.block_size);  // zeros, which a weight of zero must meet
+        if (lane >= pages || pos >= a.prefix) return outside;
+        const int page = pos / a.block_size;
+        const long long block = __ldg(a.tables + page);
+        if (block < 0 || block >= a.num_blocks) return outside;
+        return (int)(block * a.block_size + (pos - page * a.block_size));
+      };
+      int row_now = page_of(first % p.tiles);
+      for (int w = first; w < last; ++w) {
+        const int n = w - first, stage = n & 1, kv_head = w / p.tiles / a.row_tiles;
+        const int row_next = page_of((w + 1) % p.tiles);
+        for (int is_v = 0; is_v < 2; ++is_v) {
+          uint64_t *full = (is_v ? v_full : k_full) + stage, *empty = (is_v ? v_empty : k_empty) + stage;
+          wait_or_give_up(empty, ((n >> 1) & 1) ^ 1, dead);
+          if (dead) break;
+          if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
+          __syncwarp();
+          for (int i = lane; __any_sync(0xffffffffu, i < pages * (DT / 64)); i += 32) {
+            const int page = i % pages, half = i / pages;
+            const int row = __shfl_sync(0xffffffffu, row_now, page);
+            if (half < DT / 64)
+              tma_load3(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + half * S::kHalf + page * box_rows * 128,
+                        is_v ? &value_map : &key_map, half * 64, kv_head, row, full);
+          }
+        }
+        if (dead) break;
+        row_now = row_next;
+      }
+    } else if (warp == 9) {
+      if (lane == 0) {
+        // Steps of a piece: (tile t, group g) in order; the score product of a group's next step follows its own weights'
+        // product, and the other group's come between.
+        const unsigned score_kind = mma_kind<T>(kPrefixTile, false), value_kind = mma_kind<T>(DT, true);
+        int pieces[2] = {0, 0}, done[2] = {0, 0};  // per group: pieces begun, steps whose weights' products were issued
+        const auto scores = [&](int g, int n) {  // S_g = Q_g K^T with the run's n-th tile
+          const unsigned q = smem_at + g * (kGroupRows * DT * 2), k = smem_at + S::kOffK + (n & 1) * S::kTileBytes;
+  #pragma unroll
+          for (int i = 0; i < DT / 16; ++i)
+            tc_mma(tmem + g * kPrefixTile, operand(q + (i >> 2) * S::kHalf + (i & 3) * 32, 16),
+                   operand(k + (i >> 2) * S::kHalf + (i & 3) * 32, 16), score_kind, i > 0);
+          tc_commit(&s_full[g]);
+        };
+        const auto values = [&](int g, int n, bool add) {  // O_g (+)= P_g V
+          const unsigned v = smem_at + S::kOffV + (n & 1) * S::kTileBytes;
+  #pragma unroll
+          for (int i = 0; i < kPrefixTile / 16; ++i)
+            tc_mma_tmem(tmem + 2 * kPrefixTile + g * DT, tmem + g * kPrefixTile + i * 8, operand(v + i * 2048, S::kHalf), value_kind,
+                        add || i > 0);
+          tc_commit(&o_full[g]);
+        };
+        for (int w = first; w < last;) {
+          const int count = min(p.tiles - w % p.tiles, last - w), n0 = w - first;
+          const int steps = alternate ? count : 2 * count;
+          // Score products run two steps ahead of the weights' products, one for each group.
+          const auto issue_scores = [&](int step) {
+            const int g = step & 1, n = n0 + (alternate ? step : step >> 1);
+            if (step < 2) {
+              wait_or_give_up(&q_full[g], pieces[g]++ & 1, dead);
+            } else {
+              wait_or_give_up(&o_full[g], (done[g] - 1) & 1, dead);  // P_g, which lies over S_g, has been used
+            }
+            if (alternate || g == 0) wait_or_give_up(&k_full[n & 1], (n >> 1) & 1, dead);
+            tc_fence_after();
+            scores(g, n);
+            if (alternate || g == 1) tc_commit(&k_empty[n & 1]);
+          };
+          issue_scores(0);
+          if (steps > 1) issue_scores(1);
+          for (int step = 0; step < steps; ++step) {
+            const int g = step & 1, n = n0 + (alternate ? step : step >> 1);
+            if (alternate || g == 0) wait_or_give_up(&v_full[n & 1], (n >> 1) & 1, dead);
+            wait_or_give_up(&p_full[g], done[g] & 1, dead);
+            tc_fence_after();
+            values(g, n, step >= 2);
+            ++done[g];
+            if (alternate || g == 1) tc_commit(&v_empty[n & 1]);
+            if (step + 2 < steps) issue_scores(step + 2);
+          }
+          w += count;
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int g = warp >> 2, row = tid & (kGroupRows - 1);
+    const unsigned lane_at = (unsigned)((warp & 3) * 32) << 16;
+    const unsigned s_at = tmem + lane_at + g * kPrefixTile, o_at = tmem + lane_at + 2 * kPrefixTile + g * DT;
+    int step = 0;  // this group's steps so far
+    for (int w = first; w < last;) {
+      const int unit = w / p.tiles, tile0 = w - unit * p.tiles, count = min(p.tiles - tile0, last - w);
+      const int kv_head = unit / a.row_tiles;
+      const int row0 = (unit - kv_head * a.row_tiles) * p.unit_rows + (alternate ? 0 : g * kGroupRows);
+      const bool any = !alternate || g < count;  // a piece of one tile has nothing for the second group
+      // The piece's queries, in the products' layout.
+      for (int i = any ? row : kGroupRows * (DT / 8); i < kGroupRows * (DT / 8); i += kGroupRows) {
+        const int r = i / (DT / 8), chunk = i % (DT / 8);
+        const Row x = row_of<true>(a, 0, kv_head, row0 + r);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (x.real && chunk * 8 < a.head_dim)
+          v = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head +
+                                                   chunk * 8));
+        const unsigned at = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf + r * 128 + (((chunk ^ r) & 7) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      }
+      if (any) {
+        fence_proxy_async();
+        mbar_arrive(&q_full[g]);
+      }
+
+      float m = -INFINITY, l = 0.0f;
+      bool begun = false;
+      for (int t = alternate ? g : 0; t < count; t += alternate ? 2 : 1) {
+        wait_or_give_up(&s_full[g], step & 1, dead);
+        ++step;
+        tc_fence_after();
+        unsigned s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_load(s[c]);
+        const int seen = a.prefix - (tile0 + t) * kPrefixTile;  // positions of the tile
+        if (seen < kPrefixTile) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= seen) s[c][e] = __float_as_uint(-INFINITY);
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c][e]));
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        if (!begun) {
+          m = most;
+        } else if (__any_sync(0xffffffffu, most > m + kSlack)) {
+          const float rise = fmaxf(m, most), down = exp2_fast(m - (rise == -INFINITY ? 0.0f : rise));
+          m = rise;
+          l *= down;
+#pragma unroll
+          for (int c = 0; c < DT; c += 32) {
+            unsigned o[32];
+            tmem_load32(o_at + c, o);
+            tmem_wait_load(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * down);
+            tmem_store32(o_at + c, o);
+          }
+        }
+        begun = true;
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          unsigned w16[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int j = 2 * e;
+            const float x = exp2_fast(fmaf(__uint_as_float(s[2 * c + (j >> 5)][j & 31]), a.scale_log2, -ref));
+            const float y = exp2_fast(fmaf(__uint_as_float(s[2 * c + (j >> 5)][(j & 31) + 1]), a.scale_log2, -ref));
+            sum[e & 1] += x;
+            sum[2 + (e & 1)] += y;
+            w16[e] = pack2(x, y, T{});
+          }
+          tmem_store32(s_at + c * 32, w16);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_store();
+        tc_fence_before();
+        mbar_arrive(&p_full[g]);
+      }
+
+      // The piece: this thread's row of it.
+      if (any) {
+        wait_or_give_up(&o_full[g], (step - 1) & 1, dead);
+        tc_fence_after();
+      }
+      const long long slot = ((long long)unit + blockIdx.x) * 2 + g;
+      const bool real = row_of<true>(a, 0, kv_head, row0 + row).real;
+      float* dst = a.part + (slot * kGroupRows + row) * a.head_dim;
+#pragma unroll
+      for (int c = 0; c < DT; c += 32) {
+        unsigned o[32];
+        tmem_load32(o_at + c, o);
+        tmem_wait_load(o);
+        if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (c + e < a.head_dim)
+              *reinterpret_cast<uint4*>(dst + c + e) = any ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      if (real) a.ml[slot * kGroupRows + row] = make_float2(m, l);
+      tc_fence_before();  // the next piece's products may overwrite O_g once its queries are announced
+      w += count;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+}  // namespace
+}  // namespace ckb

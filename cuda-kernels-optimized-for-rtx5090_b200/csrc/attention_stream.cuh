@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kTile / box_rows;
     const int box_bytes = box_rows * 128;
     const auto page_of = [&](const Cursor& c) -> int {  // lane p: the cache row where page p of the tile begins
-      const int pos = a.prefix + c.tile * kTile + lane * box_rows;
+      const int pos = own_begin(a.prefix, a.tokens, lens[c.b]) + c.tile * kTile + lane * box_rows;
       if (lane >= pages || pos >= lens[c.b]) return -1;
       const int page = pos / a.block_size;
       const long long block = __ldg(a.tables + (long long)c.b * a.table_width + page);
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   const int wr = warp % WR, wk = warp / WR, quad_row = lane >> 2;
   constexpr int kNt = kKeys / 8, kDt = DT / 8;
   float o[kDt][4], m[2], l[2];
-  int len = 0, min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
+  int len = 0, begin = 0, min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
   for (int w = first; w < last; ++w) {
     const int stage = (w - first) % kStages;
     const int kv_head = at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
       ++q_now;
       piece_begin = at.tile;
       len = lens[at.b];
+      begin = own_begin(a.prefix, a.tokens, len);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int in = row0 + wr * 16 + quad_row + 8 * i;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
 
     const unsigned k_at = smem_at + stage * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
     const unsigned q_at = smem_at + S::kOffQ + ((q_now - 1) % kStages) * S::kQBytes;
-    const int pos0 = a.prefix + at.tile * kTile + wk * kKeys;
+    const int pos0 = begin + at.tile * kTile + wk * kKeys;
     float s[kNt][4];
 #pragma unroll
     for (int n = 0; n < kNt; ++n)
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     }
 
     if (at.tile + 1 == at.tiles || w + 1 == last) {  // the end of a piece
-      const bool whole = a.prefix == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
+      const bool whole = begin == 0 && piece_begin == 0 && at.tile + 1 == at.tiles;
       const long long slot = (long long)at.b * units + at.unit + blockIdx.x;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
