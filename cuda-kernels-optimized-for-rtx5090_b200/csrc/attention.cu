@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
 namespace ckb {
 namespace {
 
-// Joins the pieces of each output row: a warp per row (b, t, head).
+// Joins the pieces of each output row (b, t, head).
 struct JoinArgs {
   void* out;
   const long long* lens;
@@ -593,12 +593,14 @@ struct JoinArgs {
   int shared_slots, shared_split;     // slots of a piece; whether they are parts of the positions, not of the rows
 };
 
-template <typename T>
+// kWarps warps take a row's pieces in turn: 1 where there are rows enough to fill the GPU, 8 where a few rows have many pieces.
+template <typename T, int kWarps>
 __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
+  constexpr int kAhead = 8;  // pieces whose loads are in flight together
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kWarps;
+  const long long row = (long long)blockIdx.x * (8 / kWarps) + warp / kWarps;
   if (row >= (long long)a.batch * a.tokens * a.q_heads) return;
   const int head = (int)(row % a.q_heads), t = (int)(row / a.q_heads % a.tokens), b = (int)(row / a.q_heads / a.tokens);
   const int kv_head = head / a.group, in = t * a.group + (head - kv_head * a.group);
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
     const int w0 = begin + unit * tiles, c0 = w0 / run;
     own = (w0 + tiles - 1) / run - c0 + 1;
     own_at = ((long long)b * units + unit + c0) * a.own_rows + in % a.own_rows;
-    if (own == 1 && !sharing) return;  // written out by its CTA
+    if (own == 1 && !sharing) return;  // written out by its CTA (the same for all warps of the row)
   }
   int shared = 0, shared_step = 0;
   long long shared_at = 0;
@@ -632,34 +634,62 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
   }
   const auto at = [&](int i) { return i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * shared_step; };
   const int pieces = own + shared;
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, (i < own ? a.own_ml : a.shared_ml)[at(i)].x);
+  const auto ml_of = [&](int i) { return (i < own ? a.own_ml : a.shared_ml)[at(i)]; };
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, ml_of(i).x);
   top = warp_max(top);
   const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
   for (int i = lane; i < pieces; i += 32) {
-    const float2 v = (i < own ? a.own_ml : a.shared_ml)[at(i)];
+    const float2 v = ml_of(i);
     sum += v.y * exp2_fast(v.x - ref);
   }
   sum = warp_sum(sum);
   const bool some = len - a.tokens + t + 1 > 0;
+  const float inv = 1.0f / sum;
   T* out = (T*)a.out + row * a.head_dim;
-  for (int c = lane * 4; c < a.head_dim; c += 128) {
+  __shared__ float4 partial[kWarps > 1 ? 8 : 1][32];
+  for (int c0 = 0; c0 < a.head_dim; c0 += 128) {
+    const int c = c0 + lane * 4;
+    const bool inside = some && c < a.head_dim;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (some) {
-#pragma unroll 4
-      for (int i = 0; i < pieces; ++i) {
-        const float w = exp2_fast((i < own ? a.own_ml : a.shared_ml)[at(i)].x - ref);
-        const float4 v = *reinterpret_cast<const float4*>((i < own ? a.own_part : a.shared_part) + at(i) * a.head_dim + c);
-        acc.x = fmaf(w, v.x, acc.x);
-        acc.y = fmaf(w, v.y, acc.y);
-        acc.z = fmaf(w, v.z, acc.z);
-        acc.w = fmaf(w, v.w, acc.w);
+    for (int i0 = part; i0 < pieces; i0 += kAhead * kWarps) {
+      float4 v[kAhead];
+      float w[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k * kWarps;
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        w[k] = -INFINITY;
+        if (i < pieces) {
+          w[k] = ml_of(i).x;
+          if (inside) v[k] = *reinterpret_cast<const float4*>((i < own ? a.own_part : a.shared_part) + at(i) * a.head_dim + c);
+        }
       }
-      const float inv = 1.0f / sum;
-      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const float x = exp2_fast(w[k] - ref);
+        acc.x = fmaf(x, v[k].x, acc.x);
+        acc.y = fmaf(x, v[k].y, acc.y);
+        acc.z = fmaf(x, v[k].z, acc.z);
+        acc.w = fmaf(x, v[k].w, acc.w);
+      }
     }
-    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2(acc.x, acc.y, T{}), pack2(acc.z, acc.w, T{}));
+    if (kWarps > 1) {
+      partial[warp][lane] = acc;
+      __syncthreads();  // a block has one row then
+      if (part == 0) {
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) {
+          const float4 v = partial[k][lane];
+          acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+        }
+      }
+      __syncthreads();
+    }
+    if (part == 0 && c < a.head_dim) {
+      const uint2 v = make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}));
+      *reinterpret_cast<uint2*>(out + c) = some ? v : make_uint2(0u, 0u);
+    }
   }
 }
 
@@ -838,7 +868,9 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
                      a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, h.rows,
                      h.unit_rows, h.row_tiles, h.tiles, h.run, h.slots, h.unit_rows == h.rows && h.slots > 1};
     const long long rows = (long long)a.batch * a.tokens * a.q_heads;
-    err = launch_pdl(join_rows<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, j);
+    err = rows < 8LL * device_sm_count()
+              ? launch_pdl(join_rows<T, 8>, dim3((unsigned)rows), dim3(256), 0, stream, j)
+              : launch_pdl(join_rows<T, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, j);
   }
   if (err != cudaSuccess) {
     cudaGetLastError();

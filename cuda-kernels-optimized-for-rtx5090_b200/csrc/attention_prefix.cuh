@@ -9,10 +9,12 @@
 //   warps 0-3, 4-7  a softmax group each, a thread a row: scores S from TMEM, running maximum, exp, the weights P back to
 //                   TMEM in 16 bits over S, the sum of the unrounded weights in fp32;
 //   warp 8          looks the pages up and loads keys and values by TMA (rings of two tiles each);
-//   warp 9          issues S_i = Q_i K^T and O_i += P_i V (P_i from TMEM) for the two groups in turn: while one group
-//                   works on its scores, the tensor cores work for the other.
+//   warp 9          issues S = Q K^T and O += P V (P from TMEM) for the two groups in turn.
+// A step is half a tile, 64 positions, so that each group has two S buffers: while it works on one, the tensor cores fill
+// the other. (With one buffer of 128 positions a group waited 1.6 us for its next scores after 1.0 us of work on them: P,
+// which lies over S, had to be used up first.)
 // The two groups have a row tile of 128 each of a 256-row unit, or every other tile of positions of a 128-row unit (then
-// they are two pieces). O_i stays in TMEM. It is scaled down only when a row's maximum has risen by more than 8 (powers of
+// they are two pieces). O stays in TMEM. It is scaled down only when a row's maximum has risen by more than 8 (powers of
 // 2) over the one in use; until then weights may reach 2^8, which fp32 sums and 16-bit weights hold as well as 1.
 #pragma once
 
@@ -21,7 +23,8 @@ namespace {
 
 constexpr int kPrefixTile = 128;  // positions of a tile
 constexpr int kGroupRows = 128;   // query rows of a softmax group
-constexpr int kPrefixThreads = 384;  // warps 10 and 11 only fill the third warpgroup, which hands its registers over
+constexpr int kPrefixThreads = 320;
+constexpr int kStep = 64;         // positions of a step
 constexpr float kSlack = 8.0f;    // by how much a maximum may fall behind
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -114,7 +117,7 @@ struct PrefixShape {
   static constexpr int kOffK = 2 * kGroupRows * DT * 2;
   static constexpr int kOffV = kOffK + 2 * kTileBytes;
   static constexpr int kOffBars = kOffV + 2 * kTileBytes;
-  static constexpr int kBytes = kOffBars + 16 * 8 + 16 + 1024;
+  static constexpr int kBytes = kOffBars + 22 * 8 + 16 + 1024;
   static constexpr int kHalf = kPrefixTile * 128;  // bytes of 64 columns of a tile
 };
 
@@ -128,8 +131,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const unsigned smem_at = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;  // by stage
-  uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12, *o_full = bars + 14;  // by group
-  unsigned* tmem_sh = reinterpret_cast<unsigned*>(bars + 16);
+  uint64_t* q_full = bars + 8;  // by group
+  uint64_t *s_full = bars + 10, *p_full = bars + 14, *o_full = bars + 18;  // by group and buffer
+  unsigned* tmem_sh = reinterpret_cast<unsigned*>(bars + 22);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -138,17 +142,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&q_full[i], kGroupRows);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kGroupRows);
       mbar_init(&o_full[i], 1);
     }
     mbar_fence_init();
+    tma_prefetch(&key_map);
+    tma_prefetch(&value_map);
   }
   if (warp == 9) tmem_alloc(tmem_sh, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = *tmem_sh;  // columns: S_0 | S_1 (128 each, P_i over S_i), then O_0 | O_1
+  const unsigned tmem = *tmem_sh;  // columns: S of group 0 (two buffers of 64, P over S), of group 1, then O_0, O_1
   pdl_wait();
   pdl_trigger();
 
@@ -156,117 +164,124 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const bool alternate = p.unit_rows == kGroupRows;
   const int first = blockIdx.x * p.run, last = min(first + p.run, units * p.tiles);
   bool dead = false;
-  // 168 registers a thread at launch: 384 x 168 = 64512 >= 256 x 208 + 128 x 80.
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8) {
-      const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kPrefixTile / box_rows;
-      const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
-        const int pos = tile * kPrefixTile + lane * box_rows;
-        const int outside = (int)(a.num_blocks * a.block_size);  // zeros, which a weight of zero must meet
-        if (lane >= pages || pos >= a.prefix) return outside;
-        const int page = pos / a.block_size;
-        const long long block = __ldg(a.tables + page);
-        if (block < 0 || block >= a.num_blocks) return outside;
-        return (int)(block * a.block_size + (pos - page * a.block_size));
-      };
-      int row_now = page_of(first % p.tiles);
-      for (int w = first; w < last; ++w) {
-        const int n = w - first, stage = n & 1, kv_head = w / p.tiles / a.row_tiles;
-        const int row_next = page_of((w + 1) % p.tiles);
-        for (int is_v = 0; is_v < 2; ++is_v) {
-          uint64_t *full = (is_v ? v_full : k_full) + stage, *empty = (is_v ? v_empty : k_empty) + stage;
-          wait_or_give_up(empty, ((n >> 1) & 1) ^ 1, dead);
-          if (dead) break;
-          if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
-          __syncwarp();
-          for (int i = lane; __any_sync(0xffffffffu, i < pages * (DT / 64)); i += 32) {
-            const int page = i % pages, half = i / pages;
-            const int row = __shfl_sync(0xffffffffu, row_now, page);
-            if (half < DT / 64)
-              tma_load3(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + half * S::kHalf + page * box_rows * 128,
-                        is_v ? &value_map : &key_map, half * 64, kv_head, row, full);
-          }
-        }
+  if (warp == 8) {
+    const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kPrefixTile / box_rows;
+    const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
+      const int pos = tile * kPrefixTile + lane * box_rows;
+      const int outside = (int)(a.num_blocks * a.block_size);  // zeros, which a weight of zero must meet
+      if (lane >= pages || pos >= a.prefix) return outside;
+      const int page = pos / a.block_size;
+      const long long block = __ldg(a.tables + page);
+      if (block < 0 || block >= a.num_blocks) return outside;
+      return (int)(block * a.block_size + (pos - page * a.block_size));
+    };
+    int row_now = page_of(first % p.tiles);
+    for (int w = first; w < last; ++w) {
+      const int n = w - first, stage = n & 1, kv_head = w / p.tiles / a.row_tiles;
+      const int row_next = page_of((w + 1) % p.tiles);
+      for (int is_v = 0; is_v < 2; ++is_v) {
+        uint64_t *full = (is_v ? v_full : k_full) + stage, *empty = (is_v ? v_empty : k_empty) + stage;
+        wait_or_give_up(empty, ((n >> 1) & 1) ^ 1, dead);
         if (dead) break;
-        row_now = row_next;
-      }
-    } else if (warp == 9) {
-      if (lane == 0) {
-        // Steps of a piece: (tile t, group g) in order; the score product of a group's next step follows its own weights'
-        // product, and the other group's come between.
-        const unsigned score_kind = mma_kind<T>(kPrefixTile, false), value_kind = mma_kind<T>(DT, true);
-        int pieces[2] = {0, 0}, done[2] = {0, 0};  // per group: pieces begun, steps whose weights' products were issued
-        const auto scores = [&](int g, int n) {  // S_g = Q_g K^T with the run's n-th tile
-          const unsigned q = smem_at + g * (kGroupRows * DT * 2), k = smem_at + S::kOffK + (n & 1) * S::kTileBytes;
-  #pragma unroll
-          for (int i = 0; i < DT / 16; ++i)
-            tc_mma(tmem + g * kPrefixTile, operand(q + (i >> 2) * S::kHalf + (i & 3) * 32, 16),
-                   operand(k + (i >> 2) * S::kHalf + (i & 3) * 32, 16), score_kind, i > 0);
-          tc_commit(&s_full[g]);
-        };
-        const auto values = [&](int g, int n, bool add) {  // O_g (+)= P_g V
-          const unsigned v = smem_at + S::kOffV + (n & 1) * S::kTileBytes;
-  #pragma unroll
-          for (int i = 0; i < kPrefixTile / 16; ++i)
-            tc_mma_tmem(tmem + 2 * kPrefixTile + g * DT, tmem + g * kPrefixTile + i * 8, operand(v + i * 2048, S::kHalf), value_kind,
-                        add || i > 0);
-          tc_commit(&o_full[g]);
-        };
-        for (int w = first; w < last;) {
-          const int count = min(p.tiles - w % p.tiles, last - w), n0 = w - first;
-          const int steps = alternate ? count : 2 * count;
-          // Score products run two steps ahead of the weights' products, one for each group.
-          const auto issue_scores = [&](int step) {
-            const int g = step & 1, n = n0 + (alternate ? step : step >> 1);
-            if (step < 2) {
-              wait_or_give_up(&q_full[g], pieces[g]++ & 1, dead);
-            } else {
-              wait_or_give_up(&o_full[g], (done[g] - 1) & 1, dead);  // P_g, which lies over S_g, has been used
-            }
-            if (alternate || g == 0) wait_or_give_up(&k_full[n & 1], (n >> 1) & 1, dead);
-            tc_fence_after();
-            scores(g, n);
-            if (alternate || g == 1) tc_commit(&k_empty[n & 1]);
-          };
-          issue_scores(0);
-          if (steps > 1) issue_scores(1);
-          for (int step = 0; step < steps; ++step) {
-            const int g = step & 1, n = n0 + (alternate ? step : step >> 1);
-            if (alternate || g == 0) wait_or_give_up(&v_full[n & 1], (n >> 1) & 1, dead);
-            wait_or_give_up(&p_full[g], done[g] & 1, dead);
-            tc_fence_after();
-            values(g, n, step >= 2);
-            ++done[g];
-            if (alternate || g == 1) tc_commit(&v_empty[n & 1]);
-            if (step + 2 < steps) issue_scores(step + 2);
-          }
-          w += count;
+        if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
+        __syncwarp();
+        for (int i = lane; __any_sync(0xffffffffu, i < pages * (DT / 64)); i += 32) {
+          const int page = i % pages, half = i / pages;
+          const int row = __shfl_sync(0xffffffffu, row_now, page);
+          if (half < DT / 64)
+            tma_load3(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + half * S::kHalf + page * box_rows * 128,
+                      is_v ? &value_map : &key_map, half * 64, kv_head, row, full);
         }
       }
-      __syncwarp();
+      if (dead) break;
+      row_now = row_next;
     }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      // Group g's u-th step of a piece takes half u & 1 of its (u >> 1)-th tile. Scores run two steps ahead of the weights'
+      // products. Those of step u + 2 go into the buffer that step u's weights lie in, so they wait for its product, but only
+      // after the other group's next product has been issued: the tensor cores always have one to go on with.
+      const unsigned score_kind = mma_kind<T>(kStep, false), value_kind = mma_kind<T>(DT, true);
+      int pieces[2] = {0, 0};  // per group: pieces begun
+      int base[2] = {0, 0};    // per group: steps of the pieces before
+      for (int w = first; w < last;) {
+        const int count = min(p.tiles - w % p.tiles, last - w), n0 = w - first;
+        const int steps[2] = {alternate ? (count + 1) / 2 * 2 : 2 * count, alternate ? count / 2 * 2 : 2 * count};
+        const auto tile_of = [&](int g, int u) { return n0 + (alternate ? (u & ~1) + g : u >> 1); };
+        const auto scores = [&](int g, int u) {
+          const int n = tile_of(g, u), at = base[g] + u;
+          if (u == 0) wait_or_give_up(&q_full[g], pieces[g]++ & 1, dead);
+          if (u >= 2) wait_or_give_up(&o_full[g * 2 + (at & 1)], (at - 2) >> 1 & 1, dead);  // step u - 2's weights are used
+          if ((u & 1) == 0 && (alternate || g == 0)) wait_or_give_up(&k_full[n & 1], (n >> 1) & 1, dead);
+          tc_fence_after();
+          const unsigned q = smem_at + g * (kGroupRows * DT * 2);
+          const unsigned k = smem_at + S::kOffK + (n & 1) * S::kTileBytes + (u & 1) * (kStep * 128);
+#pragma unroll
+          for (int i = 0; i < DT / 16; ++i)
+            tc_mma(tmem + (g * 2 + (at & 1)) * kStep, operand(q + (i >> 2) * S::kHalf + (i & 3) * 32, 16),
+                   operand(k + (i >> 2) * S::kHalf + (i & 3) * 32, 16), score_kind, i > 0);
+          tc_commit(&s_full[g * 2 + (at & 1)]);
+          if ((u & 1) == 1 && (alternate || g == 1)) tc_commit(&k_empty[n & 1]);
+        };
+        const auto values = [&](int g, int u) {
+          const int n = tile_of(g, u), at = base[g] + u;
+          if ((u & 1) == 0 && (alternate || g == 0)) wait_or_give_up(&v_full[n & 1], (n >> 1) & 1, dead);
+          wait_or_give_up(&p_full[g * 2 + (at & 1)], (at >> 1) & 1, dead);
+          tc_fence_after();
+          const unsigned v = smem_at + S::kOffV + (n & 1) * S::kTileBytes + (u & 1) * (kStep * 128);
+#pragma unroll
+          for (int i = 0; i < kStep / 16; ++i)
+            tc_mma_tmem(tmem + 4 * kStep + g * DT, tmem + (g * 2 + (at & 1)) * kStep + i * 8, operand(v + i * 2048, S::kHalf),
+                        value_kind, u > 0 || i > 0);
+          tc_commit(&o_full[g * 2 + (at & 1)]);
+          if ((u & 1) == 1 && (alternate || g == 1)) tc_commit(&v_empty[n & 1]);
+        };
+        for (int u = 0; u < 2; ++u)
+          for (int g = 0; g < 2; ++g)
+            if (u < steps[g]) scores(g, u);
+        for (int u = 0; u < steps[0]; ++u) {  // group 0 has as many steps as group 1, or more
+          values(0, u);
+          if (u > 0 && u + 1 < steps[1]) scores(1, u + 1);
+          if (u < steps[1]) values(1, u);
+          if (u + 2 < steps[0]) scores(0, u + 2);
+        }
+        base[0] += steps[0];
+        base[1] += steps[1];
+        w += count;
+      }
+    }
+    __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = warp >> 2, row = tid & (kGroupRows - 1);
     const unsigned lane_at = (unsigned)((warp & 3) * 32) << 16;
-    const unsigned s_at = tmem + lane_at + g * kPrefixTile, o_at = tmem + lane_at + 2 * kPrefixTile + g * DT;
+    const unsigned s_at = tmem + lane_at + g * 2 * kStep, o_at = tmem + lane_at + 4 * kStep + g * DT;
     int step = 0;  // this group's steps so far
     for (int w = first; w < last;) {
       const int unit = w / p.tiles, tile0 = w - unit * p.tiles, count = min(p.tiles - tile0, last - w);
       const int kv_head = unit / a.row_tiles;
       const int row0 = (unit - kv_head * a.row_tiles) * p.unit_rows + (alternate ? 0 : g * kGroupRows);
       const bool any = !alternate || g < count;  // a piece of one tile has nothing for the second group
-      // The piece's queries, in the products' layout.
-      for (int i = any ? row : kGroupRows * (DT / 8); i < kGroupRows * (DT / 8); i += kGroupRows) {
-        const int r = i / (DT / 8), chunk = i % (DT / 8);
-        const Row x = row_of<true>(a, 0, kv_head, row0 + r);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (x.real && chunk * 8 < a.head_dim)
-          v = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head +
-                                                   chunk * 8));
-        const unsigned at = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf + r * 128 + (((chunk ^ r) & 7) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      // The piece's queries, in the products' layout. All loads go out together.
+      constexpr int kChunks = DT / 8;
+      if (any) {
+        uint4 v[kChunks];
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int r = (i * kGroupRows + row) / kChunks, chunk = row % kChunks;
+          const Row x = row_of<true>(a, 0, kv_head, row0 + r);
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (x.real && chunk * 8 < a.head_dim)
+            v[i] = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head +
+                                                        chunk * 8));
+        }
+        sync_warps(1 + g, kGroupRows);  // the last piece's rows have left these bytes
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int r = (i * kGroupRows + row) / kChunks, chunk = row % kChunks;
+          const unsigned at = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf + r * 128 + (((chunk ^ r) & 7) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
+                       : "memory");
+        }
       }
       if (any) {
         fence_proxy_async();
@@ -274,36 +289,36 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       }
 
       float m = -INFINITY, l = 0.0f;
-      bool begun = false;
-      for (int t = alternate ? g : 0; t < count; t += alternate ? 2 : 1) {
-        wait_or_give_up(&s_full[g], step & 1, dead);
-        ++step;
+      const int steps = !alternate ? 2 * count : g == 0 ? (count + 1) / 2 * 2 : count / 2 * 2;
+      for (int u = 0; u < steps; ++u, ++step) {
+        const int buffer = step & 1, tile = tile0 + (alternate ? (u & ~1) + g : u >> 1);
+        const unsigned at = s_at + buffer * kStep;
+        wait_or_give_up(&s_full[g * 2 + buffer], (step >> 1) & 1, dead);
         tc_fence_after();
-        unsigned s[4][32];
+        unsigned s[2][32];
+        tmem_load32(at, s[0]);
+        tmem_load32(at + 32, s[1]);
+        tmem_wait_load(s[0]);
+        tmem_wait_load(s[1]);
+        const int seen = a.prefix - tile * kPrefixTile - (u & 1) * kStep;  // positions of the step
+        if (seen < kStep) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, s[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_load(s[c]);
-        const int seen = a.prefix - (tile0 + t) * kPrefixTile;  // positions of the tile
-        if (seen < kPrefixTile) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e >= seen) s[c][e] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < kStep; ++e)
+            if (e >= seen) s[e >> 5][e & 31] = __float_as_uint(-INFINITY);
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[c][e]));
+        for (int e = 0; e < kStep; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[e >> 5][e & 31]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-        if (!begun) {
+        if (u == 0) {
           m = most;
         } else if (__any_sync(0xffffffffu, most > m + kSlack)) {
           const float rise = fmaxf(m, most), down = exp2_fast(m - (rise == -INFINITY ? 0.0f : rise));
           m = rise;
           l *= down;
+          // The last step's product has reached O (the one before it had, or these scores would not be there).
+          wait_or_give_up(&o_full[g * 2 + (buffer ^ 1)], (step - 1) >> 1 & 1, dead);
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DT; c += 32) {
             unsigned o[32];
@@ -314,50 +329,63 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             tmem_store32(o_at + c, o);
           }
         }
-        begun = true;
         const float ref = m == -INFINITY ? 0.0f : m;
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        unsigned w16[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          unsigned w16[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int j = 2 * e;
-            const float x = exp2_fast(fmaf(__uint_as_float(s[2 * c + (j >> 5)][j & 31]), a.scale_log2, -ref));
-            const float y = exp2_fast(fmaf(__uint_as_float(s[2 * c + (j >> 5)][(j & 31) + 1]), a.scale_log2, -ref));
-            sum[e & 1] += x;
-            sum[2 + (e & 1)] += y;
-            w16[e] = pack2(x, y, T{});
-          }
-          tmem_store32(s_at + c * 32, w16);
+        for (int e = 0; e < 32; ++e) {
+          const float x = exp2_fast(fmaf(__uint_as_float(s[e >> 4][2 * (e & 15)]), a.scale_log2, -ref));
+          const float y = exp2_fast(fmaf(__uint_as_float(s[e >> 4][2 * (e & 15) + 1]), a.scale_log2, -ref));
+          sum[e & 1] += x;
+          sum[2 + (e & 1)] += y;
+          w16[e] = pack2(x, y, T{});
         }
+        tmem_store32(at, w16);
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_store();
         tc_fence_before();
-        mbar_arrive(&p_full[g]);
+        mbar_arrive(&p_full[g * 2 + buffer]);
       }
 
       // The piece: this thread's row of it.
       if (any) {
-        wait_or_give_up(&o_full[g], (step - 1) & 1, dead);
+        wait_or_give_up(&o_full[g * 2 + ((step - 1) & 1)], (step - 1) >> 1 & 1, dead);
         tc_fence_after();
       }
       const long long slot = ((long long)unit + blockIdx.x) * 2 + g;
-      const bool real = row_of<true>(a, 0, kv_head, row0 + row).real;
-      float* dst = a.part + (slot * kGroupRows + row) * a.head_dim;
+      // The queries are used up: a quarter of their bytes takes a warp's 32 rows, half of the columns at a time, so that
+      // whole rows go out.
+      constexpr int kCols = DT / 2, kParts = kCols / 4;  // columns at a time, 16-byte chunks of them
+      const unsigned stage = smem_at + g * (kGroupRows * DT * 2) + (warp & 3) * (32 * kCols * 4);
+      const int row_first = (warp & 3) * 32, rows = a.batch * a.rows - (row0 + row_first);
 #pragma unroll
-      for (int c = 0; c < DT; c += 32) {
-        unsigned o[32];
-        tmem_load32(o_at + c, o);
-        tmem_wait_load(o);
-        if (real) {
+      for (int c0 = 0; c0 < DT; c0 += kCols) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          unsigned o[32];
+          tmem_load32(o_at + c0 + c, o);
+          tmem_wait_load(o);
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            if (c + e < a.head_dim)
-              *reinterpret_cast<uint4*>(dst + c + e) = any ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             stage + lane * (kCols * 4) + ((((c + e) >> 2) ^ (lane & (kParts - 1))) << 4)),
+                         "r"(any ? o[e] : 0u), "r"(any ? o[e + 1] : 0u), "r"(any ? o[e + 2] : 0u), "r"(any ? o[e + 3] : 0u)
+                         : "memory");
         }
+        __syncwarp();
+        float* dst = a.part + (slot * kGroupRows + row_first) * a.head_dim;
+        const int chunk = lane & (kParts - 1), c = c0 + chunk * 4;
+#pragma unroll 4
+        for (int r = lane / kParts; r < 32; r += 32 / kParts) {
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + r * (kCols * 4) + ((chunk ^ (r & (kParts - 1))) << 4)));
+          if (r < rows && c < a.head_dim) *reinterpret_cast<uint4*>(dst + (long long)r * a.head_dim + c) = v;
+        }
+        __syncwarp();
       }
-      if (real) a.ml[slot * kGroupRows + row] = make_float2(m, l);
+      if (lane < rows) a.ml[slot * kGroupRows + row] = make_float2(m, l);
       tc_fence_before();  // the next piece's products may overwrite O_g once its queries are announced
       w += count;
     }

@@ -31,6 +31,9 @@ __device__ __forceinline__ void tma_load3(unsigned dst, const CUtensorMap* map, 
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // Waits for a phase unless an earlier wait of this thread ran out: then the kernel runs on to its end without waiting
 // (its results are void, the status says so).
 __device__ __forceinline__ void wait_or_give_up(uint64_t* bar, unsigned parity, bool& dead) {
@@ -86,6 +89,8 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
       mbar_init(&empty[i], kConsumers);
     }
     mbar_fence_init();
+    tma_prefetch(&key_map);
+    tma_prefetch(&value_map);
   }
   pdl_wait();
   pdl_trigger();
@@ -305,55 +310,61 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       }
-      if (S::kKeyWarps > 1) {  // join the warps that shared the positions, in the tile's own stage
-        if ((lane & 3) == 0) {
-          ml_sh[wk * kRows + wr * 16 + quad_row] = make_float2(m[0], l[0]);
-          ml_sh[wk * kRows + wr * 16 + quad_row + 8] = make_float2(m[1], l[1]);
-        }
-        sync_warps(1, 32 * kConsumers);  // and nobody reads the tile any more
-        float* sum_o = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);
-        float weight[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = wr * 16 + quad_row + 8 * i;
-          const float mine = m[i];
-          float most = -INFINITY, sum = 0.0f;
-#pragma unroll
-          for (int k = 0; k < S::kKeyWarps; ++k) most = fmaxf(most, ml_sh[k * kRows + r].x);
-          const float ref = most == -INFINITY ? 0.0f : most;
-#pragma unroll
-          for (int k = 0; k < S::kKeyWarps; ++k) sum += ml_sh[k * kRows + r].y * exp2_fast(ml_sh[k * kRows + r].x - ref);
-          weight[i] = exp2_fast(mine - ref);
-          m[i] = most;
-          l[i] = sum;
-        }
-        for (int k = 0; k < S::kKeyWarps; ++k) {
-          if (wk == k) {
-#pragma unroll
-            for (int n = 0; n < kDt; ++n)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                float2* dst = reinterpret_cast<float2*>(sum_o + (wr * 16 + quad_row + 8 * i) * DT + n * 8 + (lane & 3) * 2);
-                float2 v = make_float2(o[n][2 * i] * weight[i], o[n][2 * i + 1] * weight[i]);
-                if (k > 0) {
-                  const float2 u = *dst;
-                  v.x += u.x;
-                  v.y += u.y;
-                }
-                *dst = v;
-                o[n][2 * i] = v.x;
-                o[n][2 * i + 1] = v.y;
-              }
-          }
-          sync_warps(1, 32 * kConsumers);
-        }
-        fence_proxy_async();
-      }
-      if (wk == S::kKeyWarps - 1) {  // the last to add holds the sums
+      if (S::kKeyWarps == 1) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           write_row<T, DT>(a, row_of<false>(a, at.b, kv_head, row0 + wr * 16 + quad_row + 8 * i), whole, lim[i] > 0,
                            slot * kRows + wr * 16 + quad_row + 8 * i, lane, o, i, m[i], l[i]);
+      } else {
+        // The warps that shared the positions leave their sums in the tile's own stage, and all 128 threads join them,
+        // 4 columns each: two barriers (adding up one warp after the other took 2.6 us a piece, this takes 0.7).
+        sync_warps(1, 32 * kConsumers);  // nobody reads the tile any more
+        float* sums = reinterpret_cast<float*>(smem + stage * 2 * S::kTileBytes);  // [key warps][rows][DT]
+        const int real = min(kRows, a.rows - row0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = wr * 16 + quad_row + 8 * i;
+          if (r < real) {
+            float* dst = sums + (wk * kRows + r) * DT + (lane & 3) * 2;
+#pragma unroll
+            for (int n = 0; n < kDt; ++n)  // pairs exchanged among the rows' tiles of 8 columns: no bank twice
+              *reinterpret_cast<float2*>(dst + ((n ^ (r & 7)) * 8)) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            if ((lane & 3) == 0) ml_sh[wk * kRows + r] = make_float2(m[i], l[i]);
+          }
+        }
+        sync_warps(1, 32 * kConsumers);
+        for (int e = tid; e < real * (DT / 4); e += 32 * kConsumers) {
+          const int r = e / (DT / 4), c = (e - r * (DT / 4)) * 4;
+          float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) most = fmaxf(most, ml_sh[k * kRows + r].x);
+          const float ref = most == -INFINITY ? 0.0f : most;
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int k = 0; k < S::kKeyWarps; ++k) {
+            const float2 v = ml_sh[k * kRows + r];
+            const float weight = exp2_fast(v.x - ref);
+            sum = fmaf(v.y, weight, sum);
+            const float4 u = *reinterpret_cast<const float4*>(sums + (k * kRows + r) * DT + (((c >> 3) ^ (r & 7)) << 3) + (c & 7));
+            acc.x = fmaf(weight, u.x, acc.x);
+            acc.y = fmaf(weight, u.y, acc.y);
+            acc.z = fmaf(weight, u.z, acc.z);
+            acc.w = fmaf(weight, u.w, acc.w);
+          }
+          if (c >= a.head_dim) continue;
+          if (whole) {
+            const Row x = row_of<false>(a, at.b, kv_head, row0 + r);
+            const bool some = len - a.tokens + x.t + 1 > 0;
+            const float inv = 1.0f / sum;
+            T* dst = (T*)a.out + (((long long)x.b * a.tokens + x.t) * a.q_heads + x.head) * a.head_dim + c;
+            *reinterpret_cast<uint2*>(dst) = some ? make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}))
+                                                  : make_uint2(0u, 0u);
+          } else {
+            *reinterpret_cast<float4*>(a.part + (slot * kRows + r) * a.head_dim + c) = acc;
+            if (c == 0) a.ml[slot * kRows + r] = make_float2(most, sum);
+          }
+        }
+        fence_proxy_async();
       }
     }
     __syncwarp();
