@@ -9,7 +9,7 @@
 //   warps 0-3, 4-7  a softmax group each, a thread a row: scores S from TMEM, running maximum, exp, the weights P back to
 //                   TMEM in 16 bits over S, the sum of the unrounded weights in fp32;
 //   warp 8          looks the pages up and loads keys and values by TMA (rings of two tiles each);
-//   warp 9          issues S = Q K^T and O += P V (P from TMEM) for the two groups in turn.
+//   warps 9, 10     issue S = Q K^T and O += P V (P from TMEM), one for each group.
 // A step is half a tile, 64 positions, so that each group has two S buffers: while it works on one, the tensor cores fill
 // the other. (With one buffer of 128 positions a group waited 1.6 us for its next scores after 1.0 us of work on them: P,
 // which lies over S, had to be used up first.)
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kPrefixTile = 128;  // positions of a tile
 constexpr int kGroupRows = 128;   // query rows of a softmax group
-constexpr int kPrefixThreads = 320;
+constexpr int kPrefixThreads = 352;
 constexpr int kStep = 64;         // positions of a step
 constexpr float kSlack = 8.0f;    // by how much a maximum may fall behind
 
@@ -41,6 +41,11 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  unsigned is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0u;
 }
 // D (+)= A B, A and B in shared memory.
 __device__ __forceinline__ void tc_mma(unsigned d, uint64_t a, uint64_t b, unsigned kind, bool add) {
@@ -105,6 +110,14 @@ __device__ __forceinline__ unsigned mma_kind(int columns, bool b_rows) {
   return 1u << 4 | type << 7 | type << 10 | (b_rows ? 1u << 16 : 0u) | (unsigned)(columns >> 3) << 17 | (128u >> 4) << 24;
 }
 
+// wait_or_give_up for a wait that decides the tensor cores' pace: it polls instead of sleeping.
+__device__ __forceinline__ void wait_quick(uint64_t* bar, unsigned parity, bool& dead) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return;
+  wait_or_give_up(bar, parity, dead);
+}
+
 struct PrefixArgs {
   Args a;
   int tiles, run;  // tiles of a unit, tiles of a CTA's run
@@ -134,13 +147,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   uint64_t* q_full = bars + 8;  // by group
   uint64_t *s_full = bars + 10, *p_full = bars + 14, *o_full = bars + 18;  // by group and buffer
   unsigned* tmem_sh = reinterpret_cast<unsigned*>(bars + 22);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const bool alternate = p.unit_rows == kGroupRows;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], alternate ? 1 : 2);  // a tile is read by one group, or by both
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], alternate ? 1 : 2);
       mbar_init(&q_full[i], kGroupRows);
     }
     for (int i = 0; i < 4; ++i) {
@@ -156,12 +170,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tmem = *tmem_sh;  // columns: S of group 0 (two buffers of 64, P over S), of group 1, then O_0, O_1
+  const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_sh, 0);  // columns: S of group 0 (two buffers of 64, P over S), of group 1, then O_0, O_1
   pdl_wait();
   pdl_trigger();
 
   const int units = a.kv_heads * a.row_tiles;
-  const bool alternate = p.unit_rows == kGroupRows;
   const int first = blockIdx.x * p.run, last = min(first + p.run, units * p.tiles);
   bool dead = false;
   if (warp == 8) {
@@ -175,13 +188,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       if (block < 0 || block >= a.num_blocks) return outside;
       return (int)(block * a.block_size + (pos - page * a.block_size));
     };
-    int row_now = page_of(first % p.tiles);
+    int row_now = page_of(first % p.tiles), in_piece = 0, uses0 = 0, uses1 = 0;
     for (int w = first; w < last; ++w) {
-      const int n = w - first, stage = n & 1, kv_head = w / p.tiles / a.row_tiles;
+      // Alternate tiles of a piece have a stage each, that of their group, so that every group meets its stage's phases
+      // one after the other.
+      const int n = w - first, kv_head = w / p.tiles / a.row_tiles;
+      if (w % p.tiles == 0) in_piece = 0;
+      const int stage = (alternate ? in_piece : n) & 1, use = stage == 0 ? uses0++ : uses1++;
+      ++in_piece;
       const int row_next = page_of((w + 1) % p.tiles);
       for (int is_v = 0; is_v < 2; ++is_v) {
         uint64_t *full = (is_v ? v_full : k_full) + stage, *empty = (is_v ? v_empty : k_empty) + stage;
-        wait_or_give_up(empty, ((n >> 1) & 1) ^ 1, dead);
+        wait_or_give_up(empty, (use & 1) ^ 1, dead);
         if (dead) break;
         if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
         __syncwarp();
@@ -196,61 +214,71 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       if (dead) break;
       row_now = row_next;
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      // Group g's u-th step of a piece takes half u & 1 of its (u >> 1)-th tile. Scores run two steps ahead of the weights'
-      // products. Those of step u + 2 go into the buffer that step u's weights lie in, so they wait for its product, but only
-      // after the other group's next product has been issued: the tensor cores always have one to go on with.
-      const unsigned score_kind = mma_kind<T>(kStep, false), value_kind = mma_kind<T>(DT, true);
-      int pieces[2] = {0, 0};  // per group: pieces begun
-      int base[2] = {0, 0};    // per group: steps of the pieces before
-      for (int w = first; w < last;) {
-        const int count = min(p.tiles - w % p.tiles, last - w), n0 = w - first;
-        const int steps[2] = {alternate ? (count + 1) / 2 * 2 : 2 * count, alternate ? count / 2 * 2 : 2 * count};
-        const auto tile_of = [&](int g, int u) { return n0 + (alternate ? (u & ~1) + g : u >> 1); };
-        const auto scores = [&](int g, int u) {
-          const int n = tile_of(g, u), at = base[g] + u;
-          if (u == 0) wait_or_give_up(&q_full[g], pieces[g]++ & 1, dead);
-          if (u >= 2) wait_or_give_up(&o_full[g * 2 + (at & 1)], (at - 2) >> 1 & 1, dead);  // step u - 2's weights are used
-          if ((u & 1) == 0 && (alternate || g == 0)) wait_or_give_up(&k_full[n & 1], (n >> 1) & 1, dead);
-          tc_fence_after();
-          const unsigned q = smem_at + g * (kGroupRows * DT * 2);
-          const unsigned k = smem_at + S::kOffK + (n & 1) * S::kTileBytes + (u & 1) * (kStep * 128);
+  } else if (warp >= 9) {
+    // The whole warp goes through this, so that addresses and descriptors stay in uniform registers; one lane issues.
+    // Its group's step u takes half u & 1 of the group's (u >> 1)-th tile. Scores run two steps ahead of the weights'
+    // products; those of step u + 2 go into the buffer that step u's weights lie in, so they wait for its product. A warp for
+    // each group: one for both spent 2300 clocks on a step of the two, mostly on waits that were over (130 clocks each).
+    const int g = warp - 9;
+    const bool leader = elect_one();
+    const unsigned score_kind = mma_kind<T>(kStep, false), value_kind = mma_kind<T>(DT, true);
+    const uint64_t q_operand = operand(smem_at + g * (kGroupRows * DT * 2), 16);
+    const uint64_t k_operand = operand(smem_at + S::kOffK, 16), v_operand = operand(smem_at + S::kOffV, S::kHalf);
+    const unsigned s_at = tmem + g * 2 * kStep, o_at = tmem + 4 * kStep + g * DT;
+    int phase = 0, pieces = 0;  // tiles of the pieces before, pieces
+    for (int w = first; w < last;) {
+      const int count = min(p.tiles - w % p.tiles, last - w), n0 = w - first;
+      const int tiles = !alternate ? count : (count + 1 - g) / 2;  // of this group
+      const auto scores = [&](auto half, int j) {
+        constexpr int h = decltype(half)::value;
+        const int stage = alternate ? g : (n0 + j) & 1, use = alternate ? phase + j : (n0 + j) >> 1;
+        if (h == 0 && j == 0) wait_quick(&q_full[g], pieces & 1, dead);
+        if (j > 0) wait_quick(&o_full[g * 2 + h], (phase + j - 1) & 1, dead);  // the buffer's last weights are used
+        if (h == 0) wait_quick(&k_full[stage], use & 1, dead);
+        tc_fence_after();
+        const uint64_t k = k_operand + ((stage * S::kTileBytes + h * (kStep * 128)) >> 4);
+        if (leader) {
 #pragma unroll
           for (int i = 0; i < DT / 16; ++i)
-            tc_mma(tmem + (g * 2 + (at & 1)) * kStep, operand(q + (i >> 2) * S::kHalf + (i & 3) * 32, 16),
-                   operand(k + (i >> 2) * S::kHalf + (i & 3) * 32, 16), score_kind, i > 0);
-          tc_commit(&s_full[g * 2 + (at & 1)]);
-          if ((u & 1) == 1 && (alternate || g == 1)) tc_commit(&k_empty[n & 1]);
-        };
-        const auto values = [&](int g, int u) {
-          const int n = tile_of(g, u), at = base[g] + u;
-          if ((u & 1) == 0 && (alternate || g == 0)) wait_or_give_up(&v_full[n & 1], (n >> 1) & 1, dead);
-          wait_or_give_up(&p_full[g * 2 + (at & 1)], (at >> 1) & 1, dead);
-          tc_fence_after();
-          const unsigned v = smem_at + S::kOffV + (n & 1) * S::kTileBytes + (u & 1) * (kStep * 128);
+            tc_mma(s_at + h * kStep, q_operand + (((i >> 2) * S::kHalf + (i & 3) * 32) >> 4),
+                   k + (((i >> 2) * S::kHalf + (i & 3) * 32) >> 4), score_kind, i > 0);
+          tc_commit(&s_full[g * 2 + h]);
+          if (h == 1) tc_commit(&k_empty[stage]);
+        }
+        __syncwarp();
+      };
+      const auto values = [&](auto half, int j) {
+        constexpr int h = decltype(half)::value;
+        const int stage = alternate ? g : (n0 + j) & 1, use = alternate ? phase + j : (n0 + j) >> 1;
+        if (h == 0) wait_quick(&v_full[stage], use & 1, dead);
+        wait_quick(&p_full[g * 2 + h], (phase + j) & 1, dead);
+        tc_fence_after();
+        const uint64_t v = v_operand + ((stage * S::kTileBytes + h * (kStep * 128)) >> 4);
+        if (leader) {
 #pragma unroll
           for (int i = 0; i < kStep / 16; ++i)
-            tc_mma_tmem(tmem + 4 * kStep + g * DT, tmem + (g * 2 + (at & 1)) * kStep + i * 8, operand(v + i * 2048, S::kHalf),
-                        value_kind, u > 0 || i > 0);
-          tc_commit(&o_full[g * 2 + (at & 1)]);
-          if ((u & 1) == 1 && (alternate || g == 1)) tc_commit(&v_empty[n & 1]);
-        };
-        for (int u = 0; u < 2; ++u)
-          for (int g = 0; g < 2; ++g)
-            if (u < steps[g]) scores(g, u);
-        for (int u = 0; u < steps[0]; ++u) {  // group 0 has as many steps as group 1, or more
-          values(0, u);
-          if (u > 0 && u + 1 < steps[1]) scores(1, u + 1);
-          if (u < steps[1]) values(1, u);
-          if (u + 2 < steps[0]) scores(0, u + 2);
+            tc_mma_tmem(o_at, s_at + h * kStep + i * 8, v + ((i * 2048) >> 4), value_kind, h > 0 || i > 0 || j > 0);
+          tc_commit(&o_full[g * 2 + h]);
+          if (h == 1) tc_commit(&v_empty[stage]);
         }
-        base[0] += steps[0];
-        base[1] += steps[1];
-        w += count;
+        __syncwarp();
+      };
+      constexpr std::integral_constant<int, 0> zero{};
+      constexpr std::integral_constant<int, 1> one{};
+      if (tiles > 0) {
+        scores(zero, 0);
+        scores(one, 0);
+        for (int j = 0; j < tiles; ++j) {
+          values(zero, j);
+          if (j + 1 < tiles) scores(zero, j + 1);
+          values(one, j);
+          if (j + 1 < tiles) scores(one, j + 1);
+        }
+        ++pieces;
       }
+      phase += tiles;
+      w += count;
     }
-    __syncwarp();
   } else {
     const int g = warp >> 2, row = tid & (kGroupRows - 1);
     const unsigned lane_at = (unsigned)((warp & 3) * 32) << 16;
@@ -293,7 +321,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       for (int u = 0; u < steps; ++u, ++step) {
         const int buffer = step & 1, tile = tile0 + (alternate ? (u & ~1) + g : u >> 1);
         const unsigned at = s_at + buffer * kStep;
-        wait_or_give_up(&s_full[g * 2 + buffer], (step >> 1) & 1, dead);
+        wait_quick(&s_full[g * 2 + buffer], (step >> 1) & 1, dead);
         tc_fence_after();
         unsigned s[2][32];
         tmem_load32(at, s[0]);
