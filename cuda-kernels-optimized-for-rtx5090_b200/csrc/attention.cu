@@ -132,15 +132,6 @@ __device__ __forceinline__ bool not_finite(unsigned tile, int row0, int lane) {
   return __any_sync(0xffffffffu, bad);
 }
 
-// The same for a tile of 64-column halves.
-template <typename T, int DT, int kCount>
-__device__ __forceinline__ bool not_finite_box(unsigned tile, int row0, int lane) {
-  bool bad = false;
-#pragma unroll
-  for (int half = 0; half < DT / 64; ++half) bad |= not_finite<T, 64, kCount>(tile + half * (kTile * 128), row0, lane);
-  return bad;
-}
-
 // The rows of a unit: row r of the tile is query (b, t, head), or nothing.
 struct Row {
   int b, t, head;  // head: of the q heads
@@ -762,7 +753,10 @@ cudaError_t start(const Args& a, int ctas, cudaStream_t stream) {
   return launch_pdl(attend_tiles<T, DT, WR, kShared>, dim3(ctas), dim3(kThreads), bytes, stream, a);
 }
 
-// The cache as a TMA reads it: [rows][kv_heads][head_dim], boxes of box_rows rows of one head's 64 columns.
+// Whether a head has the columns of a tile, so that a box brings whole rows; else the tile's last columns are filled up.
+bool whole_rows(const Args& a) { return a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256; }
+// The cache as a TMA reads it: [kv_heads][blocks of 64 columns][rows][64], boxes of box_rows rows of one head (where they
+// are not 64, 128 or 256 columns: [kv_heads][1][rows][head_dim], boxes of 64 columns).
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -783,13 +777,15 @@ template <typename T>
 bool cache_map(const Args& a, const void* cache, int box_rows, CUtensorMap& map) {
   const EncodeTiled encode = encode_tiled();
   if (encode == nullptr) return false;
-  const cuuint64_t rows = (cuuint64_t)a.num_blocks * a.block_size;
-  const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.kv_heads, rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.head_dim * a.kv_heads * 2};
-  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
+  const cuuint64_t rows = (cuuint64_t)a.num_blocks * a.block_size, row_bytes = (cuuint64_t)a.head_dim * a.kv_heads * 2;
+  const bool whole = whole_rows(a);
+  const cuuint64_t dims[4] = {whole ? 64 : (cuuint64_t)a.head_dim, rows, whole ? (cuuint64_t)a.head_dim / 64 : 1,
+                              (cuuint64_t)a.kv_heads};
+  const cuuint64_t strides[3] = {row_bytes, 128, (cuuint64_t)a.head_dim * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)dims[2], 1}, step[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type =
       sizeof(T) == 2 && std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return encode(&map, type, 3, const_cast<void*>(cache), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return encode(&map, type, 4, const_cast<void*>(cache), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // Whether boxes of whole pages, or of 64 rows of a page, make up a tile (see attention_stream.cuh).
@@ -798,26 +794,36 @@ bool boxes_fit(const Args& a) {
          a.num_blocks * a.block_size < INT_MAX;
 }
 
+struct Maps {
+  bool fit;
+  int rows_log;  // rows of a box
+  CUtensorMap keys, values;
+};
+
+template <typename T>
+Maps maps_of(const Args& a, int rows_log) {
+  Maps m;
+  m.rows_log = rows_log;
+  m.fit = boxes_fit(a) && cache_map<T>(a, a.key, 1 << rows_log, m.keys) && cache_map<T>(a, a.value, 1 << rows_log, m.values);
+  return m;
+}
+
 template <typename T, int DT, int WR>
-cudaError_t start_stream(const Args& a, int ctas, const CUtensorMap& keys, const CUtensorMap& values, cudaStream_t stream) {
+cudaError_t start_stream(const Args& a, int ctas, const Maps& maps, cudaStream_t stream) {
   const int bytes = Ring<DT, WR>::bytes(a.batch);
   const cudaError_t err =
       cudaFuncSetAttribute(attend_stream<T, DT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attend_stream<T, DT, WR>, dim3(ctas), dim3(32 * (kConsumers + 1)), bytes, stream, a, keys, values);
+  return launch_pdl(attend_stream<T, DT, WR>, dim3(ctas), dim3(32 * (kConsumers + 1)), bytes, stream, a, maps.rows_log,
+                    maps.keys, maps.values);
 }
-
-struct Maps {
-  bool fit;
-  CUtensorMap keys, values;
-};
 
 template <typename T, int DT>
 cudaError_t start_own(const Args& a, int warps, int ctas, const Maps& maps, cudaStream_t stream) {
   if (maps.fit) {
-    if (warps == 1) return start_stream<T, DT, 1>(a, ctas, maps.keys, maps.values, stream);
-    if (warps == 2) return start_stream<T, DT, 2>(a, ctas, maps.keys, maps.values, stream);
-    return start_stream<T, DT, 4>(a, ctas, maps.keys, maps.values, stream);
+    if (warps == 1) return start_stream<T, DT, 1>(a, ctas, maps, stream);
+    if (warps == 2) return start_stream<T, DT, 2>(a, ctas, maps, stream);
+    return start_stream<T, DT, 4>(a, ctas, maps, stream);
   }
   if (warps == 1) return start<T, DT, 1, false>(a, ctas, stream);
   if (warps == 2) return start<T, DT, 2, false>(a, ctas, stream);
@@ -825,21 +831,23 @@ cudaError_t start_own(const Args& a, int warps, int ctas, const Maps& maps, cuda
 }
 
 template <typename T, int DT>
-cudaError_t start_prefix(const Args& a, const Sizes& z, const Maps& maps, cudaStream_t stream) {
+cudaError_t start_prefix(const Args& a, const Sizes& z, cudaStream_t stream) {
+  const Maps maps = maps_of<T>(a, a.block_size == 8 ? 3 : 4);
+  if (!maps.fit) return cudaErrorInvalidValue;
   const auto& h = z.shared[0];
   const int bytes = PrefixShape<DT>::kBytes;
   const cudaError_t err = cudaFuncSetAttribute(attend_prefix<T, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err != cudaSuccess) return err;
-  const PrefixArgs p{a, h.tiles, h.run, h.unit_rows};
+  const PrefixArgs p{a, h.tiles, h.run, h.unit_rows, maps.rows_log};
   return launch_pdl(attend_prefix<T, DT>, dim3(h.ctas), dim3(kPrefixThreads), bytes, stream, p, maps.keys, maps.values);
 }
 
 template <typename T>
 int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) {
   const int dt = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
-  const int box_rows = a.block_size < kTile ? a.block_size : kTile;
-  Maps maps;
-  maps.fit = boxes_fit(a) && cache_map<T>(a, a.key, box_rows, maps.keys) && cache_map<T>(a, a.value, box_rows, maps.values);
+  int rows_log = 3;  // a page, at most a tile's rows
+  while (rows_log < 6 && 2 << rows_log <= a.block_size) ++rows_log;
+  const Maps maps = maps_of<T>(a, rows_log);
   // Two groups' O and S of 256 columns each do not fit TMEM: heads of more than 128 columns take attend_tiles.
   const bool tensor = maps.fit && dt <= 128;
   const auto& h = z.shared[tensor ? 0 : 1];
@@ -853,7 +861,7 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
   s.ml = reinterpret_cast<float2*>(work + z.off_shared_ml);
   if (a.prefix > 0) {
     if (tensor)
-      err = dt == 64 ? start_prefix<T, 64>(s, z, maps, stream) : start_prefix<T, 128>(s, z, maps, stream);
+      err = dt == 64 ? start_prefix<T, 64>(s, z, stream) : start_prefix<T, 128>(s, z, stream);
     else
       err = dt == 64 ? start<T, 64, 4, true>(s, h.ctas, stream)
             : dt == 128 ? start<T, 128, 4, true>(s, h.ctas, stream)

@@ -97,11 +97,11 @@ __device__ __forceinline__ void tmem_wait_load(unsigned (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand with the 128-byte swizzle: 8 rows of 128 bytes are 1024 bytes apart (stride); `lead` is the distance
+// Shared-memory operand with the 128-byte swizzle: groups of 8 rows of 128 bytes are `stride` apart; `lead` is the distance
 // of the next 64 columns of an operand whose rows run along the sum (values), unused for one whose columns do (queries, keys).
-__device__ __forceinline__ uint64_t operand(unsigned at, unsigned lead) {
-  return (uint64_t)((at >> 4) & 0x3fffu) | (uint64_t)((lead >> 4) & 0x3fffu) << 16 | (uint64_t)(1024u >> 4) << 32 | 1ull << 46 |
-         2ull << 61;
+__device__ __forceinline__ uint64_t operand(unsigned at, unsigned lead, unsigned stride) {
+  return (uint64_t)((at >> 4) & 0x3fffu) | (uint64_t)((lead >> 4) & 0x3fffu) << 16 | (uint64_t)((stride >> 4) & 0x3fffu) << 32 |
+         1ull << 46 | 2ull << 61;
 }
 // Instruction descriptor: fp32 sums, A and B of T, 128 rows, `columns` columns, B's rows along the sum where `b_rows`.
 template <typename T>
@@ -118,10 +118,17 @@ __device__ __forceinline__ void wait_quick(uint64_t* bar, unsigned parity, bool&
   wait_or_give_up(bar, parity, dead);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 struct PrefixArgs {
   Args a;
   int tiles, run;  // tiles of a unit, tiles of a CTA's run
   int unit_rows;   // 256: the groups have 128 rows each; 128: they have every other tile each
+  int rows_log;    // rows of a box: 8 or 16
 };
 
 template <int DT>
@@ -130,7 +137,8 @@ struct PrefixShape {
   static constexpr int kOffK = 2 * kGroupRows * DT * 2;
   static constexpr int kOffV = kOffK + 2 * kTileBytes;
   static constexpr int kOffBars = kOffV + 2 * kTileBytes;
-  static constexpr int kBytes = kOffBars + 22 * 8 + 16 + 1024;
+  static constexpr int kOffRows = kOffBars + 22 * 8 + 16;
+  static constexpr int kBytes = kOffRows + 2 * kGroupRows * 8 + 1024;
   static constexpr int kHalf = kPrefixTile * 128;  // bytes of 64 columns of a tile
 };
 
@@ -178,7 +186,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const int first = blockIdx.x * p.run, last = min(first + p.run, units * p.tiles);
   bool dead = false;
   if (warp == 8) {
-    const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kPrefixTile / box_rows;
+    const int box_rows = 1 << p.rows_log, pages = kPrefixTile >> p.rows_log, blocks = a.head_dim == DT ? 1 : DT / 64;
+    const int page_bytes = box_rows * 128 * (DT / 64);
     const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
       const int pos = tile * kPrefixTile + lane * box_rows;
       const int outside = (int)(a.num_blocks * a.block_size);  // zeros, which a weight of zero must meet
@@ -203,12 +212,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (dead) break;
         if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
         __syncwarp();
-        for (int i = lane; __any_sync(0xffffffffu, i < pages * (DT / 64)); i += 32) {
-          const int page = i % pages, half = i / pages;
+        for (int i = lane; __any_sync(0xffffffffu, i < pages * blocks); i += 32) {
+          const int page = i % pages, block = i / pages;
           const int row = __shfl_sync(0xffffffffu, row_now, page);
-          if (half < DT / 64)
-            tma_load3(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + half * S::kHalf + page * box_rows * 128,
-                      is_v ? &value_map : &key_map, half * 64, kv_head, row, full);
+          if (block < blocks)
+            tma_load4(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + page * page_bytes + block * (box_rows * 128),
+                      is_v ? &value_map : &key_map, block * 64, row, kv_head, full);
         }
       }
       if (dead) break;
@@ -222,8 +231,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int g = warp - 9;
     const bool leader = elect_one();
     const unsigned score_kind = mma_kind<T>(kStep, false), value_kind = mma_kind<T>(DT, true);
-    const uint64_t q_operand = operand(smem_at + g * (kGroupRows * DT * 2), 16);
-    const uint64_t k_operand = operand(smem_at + S::kOffK, 16), v_operand = operand(smem_at + S::kOffV, S::kHalf);
+    // Keys and values lie box by box: [box][64 columns][rows of the box][128 bytes]. A step of 64 positions is 8 groups of 8
+    // rows at one distance: the first (second) 8 rows of each of the 8 boxes of 16, or the first (second) 8 boxes of 8. The
+    // order of the positions within a tile does not matter, as keys and values have the same.
+    const unsigned block = 128u << p.rows_log, box = block * (DT / 64), step = p.rows_log == 4 ? 1024u : 8u * box;
+    const uint64_t q_operand = operand(smem_at + g * (kGroupRows * DT * 2), 16, 1024);
+    const uint64_t k_operand = operand(smem_at + S::kOffK, 16, box), v_operand = operand(smem_at + S::kOffV, block, box);
     const unsigned s_at = tmem + g * 2 * kStep, o_at = tmem + 4 * kStep + g * DT;
     int phase = 0, pieces = 0;  // tiles of the pieces before, pieces
     for (int w = first; w < last;) {
@@ -236,12 +249,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (j > 0) wait_quick(&o_full[g * 2 + h], (phase + j - 1) & 1, dead);  // the buffer's last weights are used
         if (h == 0) wait_quick(&k_full[stage], use & 1, dead);
         tc_fence_after();
-        const uint64_t k = k_operand + ((stage * S::kTileBytes + h * (kStep * 128)) >> 4);
+        const uint64_t k = k_operand + ((stage * S::kTileBytes + h * step) >> 4);
         if (leader) {
 #pragma unroll
           for (int i = 0; i < DT / 16; ++i)
             tc_mma(s_at + h * kStep, q_operand + (((i >> 2) * S::kHalf + (i & 3) * 32) >> 4),
-                   k + (((i >> 2) * S::kHalf + (i & 3) * 32) >> 4), score_kind, i > 0);
+                   k + (((i >> 2) * block + (i & 3) * 32) >> 4), score_kind, i > 0);
           tc_commit(&s_full[g * 2 + h]);
           if (h == 1) tc_commit(&k_empty[stage]);
         }
@@ -253,11 +266,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (h == 0) wait_quick(&v_full[stage], use & 1, dead);
         wait_quick(&p_full[g * 2 + h], (phase + j) & 1, dead);
         tc_fence_after();
-        const uint64_t v = v_operand + ((stage * S::kTileBytes + h * (kStep * 128)) >> 4);
+        const uint64_t v = v_operand + ((stage * S::kTileBytes + h * step) >> 4);
         if (leader) {
 #pragma unroll
           for (int i = 0; i < kStep / 16; ++i)
-            tc_mma_tmem(o_at, s_at + h * kStep + i * 8, v + ((i * 2048) >> 4), value_kind, h > 0 || i > 0 || j > 0);
+            tc_mma_tmem(o_at, s_at + h * kStep + i * 8, v + ((i * 2 * box) >> 4), value_kind, h > 0 || i > 0 || j > 0);
           tc_commit(&o_full[g * 2 + h]);
           if (h == 1) tc_commit(&v_empty[stage]);
         }
@@ -283,6 +296,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int g = warp >> 2, row = tid & (kGroupRows - 1);
     const unsigned lane_at = (unsigned)((warp & 3) * 32) << 16;
     const unsigned s_at = tmem + lane_at + g * 2 * kStep, o_at = tmem + lane_at + 4 * kStep + g * DT;
+    long long* row_offset = reinterpret_cast<long long*>(smem + S::kOffRows) + g * kGroupRows;
     int step = 0;  // this group's steps so far
     for (int w = first; w < last;) {
       const int unit = w / p.tiles, tile0 = w - unit * p.tiles, count = min(p.tiles - tile0, last - w);
@@ -292,20 +306,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // The piece's queries, in the products' layout. All loads go out together.
       constexpr int kChunks = DT / 8;
       if (any) {
+        const Row mine = row_of<true>(a, 0, kv_head, row0 + row);
+        sync_warps(1 + g, kGroupRows);  // the last piece's rows have left these bytes, and their offsets are read
+        row_offset[row] = mine.real ? mine.b * a.vq.batch + mine.t * a.vq.token + mine.head * a.vq.head : -1;
+        sync_warps(1 + g, kGroupRows);
+        const int chunk = row % kChunks;
+        const T* q = (const T*)a.q + chunk * 8;
         uint4 v[kChunks];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-          const int r = (i * kGroupRows + row) / kChunks, chunk = row % kChunks;
-          const Row x = row_of<true>(a, 0, kv_head, row0 + r);
+          const long long off = row_offset[(i * kGroupRows + row) / kChunks];
           v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (x.real && chunk * 8 < a.head_dim)
-            v[i] = __ldg(reinterpret_cast<const uint4*>((const T*)a.q + x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head +
-                                                        chunk * 8));
+          if (off >= 0 && chunk * 8 < a.head_dim) v[i] = __ldg(reinterpret_cast<const uint4*>(q + off));
         }
-        sync_warps(1 + g, kGroupRows);  // the last piece's rows have left these bytes
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-          const int r = (i * kGroupRows + row) / kChunks, chunk = row % kChunks;
+          const int r = (i * kGroupRows + row) / kChunks;
           const unsigned at = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf + r * 128 + (((chunk ^ r) & 7) << 4);
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                        : "memory");
@@ -328,15 +344,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         tmem_load32(at + 32, s[1]);
         tmem_wait_load(s[0]);
         tmem_wait_load(s[1]);
-        const int seen = a.prefix - tile * kPrefixTile - (u & 1) * kStep;  // positions of the step
-        if (seen < kStep) {
+        const int seen = a.prefix - tile * kPrefixTile;  // positions of the tile: whole boxes
+        if (seen < kPrefixTile) {
 #pragma unroll
-          for (int e = 0; e < kStep; ++e)
-            if (e >= seen) s[e >> 5][e & 31] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < kStep; e += 8) {
+            const int pos = p.rows_log == 4 ? 2 * e : (u & 1) * kStep + e;  // of the group's box
+#pragma unroll
+            for (int k = e; k < e + 8; ++k)
+              if (pos >= seen) s[k >> 5][k & 31] = __float_as_uint(-INFINITY);
+          }
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < kStep; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[e >> 5][e & 31]));
+        for (int e = 0; e < kStep; e += 2)
+          top[(e >> 1) & 3] = max3(top[(e >> 1) & 3], __uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         if (u == 0) {
           m = most;
@@ -358,18 +379,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         unsigned w16[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = exp2_fast(fmaf(__uint_as_float(s[e >> 4][2 * (e & 15)]), a.scale_log2, -ref));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[e >> 4][2 * (e & 15) + 1]), a.scale_log2, -ref));
-          sum[e & 1] += x;
-          sum[2 + (e & 1)] += y;
-          w16[e] = pack2(x, y, T{});
+          const float2 pair = make_float2(__uint_as_float(s[e >> 4][2 * (e & 15)]), __uint_as_float(s[e >> 4][2 * (e & 15) + 1]));
+          float2 x = __ffma2_rn(pair, scale2, ref2);
+          x.x = exp2_fast(x.x);
+          x.y = exp2_fast(x.y);
+          sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+          w16[e] = pack2(x.x, x.y, T{});
         }
         tmem_store32(at, w16);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        sum[0] = __fadd2_rn(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_wait_store();
         tc_fence_before();
         mbar_arrive(&p_full[g * 2 + buffer]);

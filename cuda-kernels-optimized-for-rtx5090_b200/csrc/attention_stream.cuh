@@ -6,8 +6,11 @@
 // warp looks the pages up and issues a TMA box for each page and 64 columns, and the four others only multiply; each
 // goes on as soon as a tile has arrived (mbarriers), whatever the others do.
 //
-// A box is one page (or a 64-row part of one), so the block size has to divide 64 or be a multiple of it, in steps of 8
-// rows (the swizzle's period); other block sizes, and caches of 2^31 rows, go through attend_tiles.
+// A box is one page (or a 64-row part of one) with all columns of a head, as blocks of 64 columns one after the other. Few
+// large boxes matter: the TMA took about 70 clocks for each box of 16 rows and 64 columns, 2 KB, which held this kernel to
+// 5.2 TB/s and the prefix's to 4 TB/s of L2. Heads of other than 64, 128 or 256 columns take a box for each block
+// (the columns that they lack are filled up with zeros). The block size has to divide 64 or be a multiple of it, in steps of 8 rows (the
+// swizzle's period); other block sizes, and caches of 2^31 rows, go through attend_tiles.
 #pragma once
 
 #include <cuda.h>
@@ -24,11 +27,11 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void mbar_arrive_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tma_load3(unsigned dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap* map, int x, int row, int head, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
           dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(0), "r"(head)
       : "memory");
 }
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
@@ -45,10 +48,29 @@ __device__ __forceinline__ void wait_or_give_up(uint64_t* bar, unsigned parity, 
 }
 __device__ __forceinline__ void sync_warps(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// A tile in shared memory: DT / 64 halves of [64 rows][128 bytes], 16-byte chunks exchanged within a row as the TMA's
-// 128-byte swizzle does. Byte offset of chunk c (of the whole row) of row r.
-__device__ __forceinline__ unsigned at_box(int r, int c) {
-  return (c >> 3) * (kTile * 128) + r * 128 + (((c ^ r) & 7) << 4);
+// A tile in shared memory: boxes of R = 2^rows_log rows, each DT / 64 blocks of [R][128 bytes], 16-byte chunks exchanged
+// within 128 bytes as the TMA's 128-byte swizzle does. Byte offset of chunk c (of the whole row) of row r: row_part + chunk_part.
+template <int DT>
+__device__ __forceinline__ unsigned row_part(int r, int rows_log) {
+  return (((r >> rows_log) * (DT / 64) << rows_log) + (r & ((1 << rows_log) - 1))) * 128;
+}
+__device__ __forceinline__ unsigned chunk_part(int r, int c, int rows_log) {
+  return ((c >> 3) << rows_log) * 128 + (((c ^ r) & 7) << 4);
+}
+template <int DT>
+__device__ __forceinline__ unsigned at_box(int r, int c, int rows_log) {
+  return row_part<DT>(r, rows_log) + chunk_part(r, c, rows_log);
+}
+// Whether any value of rows row0 .. row0 + kCount - 1 of such a tile is infinite or NaN (the whole warp asks).
+template <typename T, int DT, int kCount>
+__device__ __forceinline__ bool not_finite_box(unsigned tile, int row0, int lane, int rows_log) {
+  bool bad = false;
+  for (int i = lane; i < kCount * (DT / 2); i += 32) {
+    const int r = i / (DT / 2), w = i % (DT / 2);
+    const float2 v = load2(tile + at_box<DT>(row0 + r, w >> 2, rows_log) + (w & 3) * 4, T{});
+    bad |= !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY);
+  }
+  return __any_sync(0xffffffffu, bad);
 }
 
 constexpr int kConsumers = 4;  // warps that multiply; one more loads
@@ -70,7 +92,7 @@ struct Ring {
 
 template <typename T, int DT, int WR>
 __global__ void __launch_bounds__(32 * (kConsumers + 1))
-    attend_stream(const Args a, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
+    attend_stream(const Args a, int rows_log, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
   using S = Ring<DT, WR>;
   constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages, kHalves = DT / 64;
   constexpr int kAll = 32 * (kConsumers + 1);
@@ -109,9 +131,9 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   bool dead = false;
 
   if (warp == kConsumers) {
-    // Pages of a tile: box_rows rows each.
-    const int box_rows = a.block_size < kTile ? a.block_size : kTile, pages = kTile / box_rows;
-    const int box_bytes = box_rows * 128;
+    // Pages of a tile: box_rows rows each, in `blocks` boxes.
+    const int box_rows = 1 << rows_log, pages = kTile >> rows_log, blocks = a.head_dim == DT ? 1 : DT / 64;
+    const int page_bytes = box_rows * 128 * (DT / 64);
     const auto page_of = [&](const Cursor& c) -> int {  // lane p: the cache row where page p of the tile begins
       const int pos = own_begin(a.prefix, a.tokens, lens[c.b]) + c.tile * kTile + lane * box_rows;
       if (lane >= pages || pos >= lens[c.b]) return -1;
@@ -131,13 +153,13 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
       wait_or_give_up(&empty[stage], (((w - first) / kStages) & 1) ^ 1, dead);
       if (dead) return;
       const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], there * box_bytes * kHalves * 2);
-      for (int i = lane; __any_sync(0xffffffffu, i < pages * kHalves * 2); i += 32) {
-        const int page = i % pages, half = i / pages % kHalves, is_v = i / (pages * kHalves);
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], there * 2 * page_bytes);
+      for (int i = lane; __any_sync(0xffffffffu, i < pages * blocks * 2); i += 32) {
+        const int page = i % pages, block = i / pages % blocks, is_v = i / (pages * blocks);
         const int row = __shfl_sync(0xffffffffu, row_now, page);
-        if (i < pages * kHalves * 2 && row >= 0)
-          tma_load3(smem_at + (stage * 2 + is_v) * S::kTileBytes + half * (kTile * 128) + page * box_bytes,
-                    is_v ? &value_map : &key_map, half * 64, kv_head, row, &full[stage]);
+        if (i < pages * blocks * 2 && row >= 0)
+          tma_load4(smem_at + (stage * 2 + is_v) * S::kTileBytes + page * page_bytes + block * (box_rows * 128),
+                    is_v ? &value_map : &key_map, block * 64, row, kv_head, &full[stage]);
       }
       if (w == first || at.tile == 0) {  // a piece begins: its queries come with its first tile
         const int row0 = (at.unit - kv_head * a.row_tiles) * kRows;
@@ -162,6 +184,12 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   }
 
   const int wr = warp % WR, wk = warp / WR, quad_row = lane >> 2;
+  unsigned k_row[kKeys / 16], v_row[kKeys / 16];  // this lane's rows of the fragments
+#pragma unroll
+  for (int n = 0; n < kKeys / 16; ++n) {
+    k_row[n] = row_part<DT>(wk * kKeys + n * 16 + (lane >> 4) * 8 + (lane & 7), rows_log);
+    v_row[n] = row_part<DT>(wk * kKeys + n * 16 + (lane & 15), rows_log);
+  }
   constexpr int kNt = kKeys / 8, kDt = DT / 8;
   float o[kDt][4], m[2], l[2];
   int len = 0, begin = 0, min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
@@ -203,7 +231,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
 #pragma unroll
       for (int n = 0; n < kNt; n += 2) {
         unsigned kb[4];
-        ldsm4(kb, k_at + at_box(wk * kKeys + n * 8 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
+        ldsm4(kb, k_at + k_row[n / 2] + chunk_part(lane & 7, 2 * k + ((lane >> 3) & 1), rows_log));
         mma(s[n], qa, kb[0], kb[1], T{});
         mma(s[n + 1], qa, kb[2], kb[3], T{});
       }
@@ -256,13 +284,13 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
       for (int i = lane; i < kKeys * (DT / 8); i += 32) {
         const int r = i / (DT / 8);
         if (pos0 + r >= len)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + at_box(wk * kKeys + r, i % (DT / 8))), "r"(0u)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + at_box<DT>(wk * kKeys + r, i % (DT / 8), rows_log)), "r"(0u)
                        : "memory");
       }
       __syncwarp();
       fence_proxy_async();  // before the ring's next copy into these bytes
     }
-    if (masked && a.tokens > 1 && not_finite_box<T, DT, kKeys>(v_at, wk * kKeys, lane)) {
+    if (masked && a.tokens > 1 && not_finite_box<T, DT, kKeys>(v_at, wk * kKeys, lane, rows_log)) {
       // A value that some row must not see is not finite: 0 * v would carry it over. One position after the other.
 #pragma unroll
       for (int n = 0; n < kNt; ++n)
@@ -273,7 +301,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
           const bool see0 = pos0 + key < lim[0], see1 = pos0 + key < lim[1];
 #pragma unroll
           for (int c = 0; c < kDt; ++c) {
-            const float2 v = load2(v_at + at_box(wk * kKeys + key, c) + (lane & 3) * 4, T{});
+            const float2 v = load2(v_at + at_box<DT>(wk * kKeys + key, c, rows_log) + (lane & 3) * 4, T{});
             if (see0) {
               o[c][0] = fmaf(p0, v.x, o[c][0]);
               o[c][1] = fmaf(p0, v.y, o[c][1]);
@@ -295,7 +323,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
 #pragma unroll
         for (int n = 0; n < kDt; n += 2) {
           unsigned vb[4];
-          ldsm4_trans(vb, v_at + at_box(wk * kKeys + k * 16 + (lane & 15), n + (lane >> 4)));
+          ldsm4_trans(vb, v_at + v_row[k] + chunk_part(lane & 7, n + (lane >> 4), rows_log));
           mma(o[n], pa, vb[0], vb[1], T{});
           mma(o[n + 1], pa, vb[2], vb[3], T{});
         }

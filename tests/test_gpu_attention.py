@@ -85,6 +85,7 @@ OWN = [  # dtype, T, Hq, Hkv, D, block size, lengths
     (BF, 1, 8, 2, 128, 8, [100, 9, 64]),
     (HF, 2, 8, 2, 64, 256, [300, 65, 513]),
     (BF, 1, 8, 2, 136, 24, [100, 9]),
+    (BF, 1, 4, 2, 192, 32, [100, 9, 65]),  # three of four blocks of columns
     (BF, 1, 2, 2, 64, 16, [i % 130 for i in range(600)]),  # more sequences than threads
 ]
 
@@ -106,6 +107,10 @@ SHARED = [  # dtype, T, Hq, Hkv, D, block size, prefix, lengths in all
     (HF, 2, 64, 1, 64, 64, 4096, [4100, 4098]),
     (BF, 1, 16, 2, 128, 128, 1024, [1024 + 7 * i for i in range(40)]),  # 320 rows a key head
     (BF, 8, 32, 4, 128, 64, 640, [648 + i for i in range(9)]),  # 576 rows a key head
+    (BF, 1, 8, 2, 128, 8, 328, [330 + i for i in range(50)]),  # boxes of 8 rows
+    (HF, 1, 16, 2, 64, 8, 1000, [1001 + i for i in range(40)]),
+    (BF, 1, 8, 2, 96, 16, 272, [280, 300]),
+    (BF, 1, 160, 160, 64, 16, 144, [145, 160]),  # more units than CTAs
 ]
 
 
