@@ -8,7 +8,7 @@
 // other units of the head. So the products and the exponentials have to run at the same time, and do:
 //   warps 0-3, 4-7  a softmax group each, a thread a row: scores S from TMEM, running maximum, exp, the weights P back to
 //                   TMEM in 16 bits over S, the sum of the unrounded weights in fp32;
-//   warp 8          looks the pages up and loads keys and values by TMA (rings of two tiles each);
+//   warps 8, 11     look the pages up and load keys and values by TMA, one each (rings of two tiles);
 //   warps 9, 10     issue S = Q K^T and O += P V (P from TMEM), one for each group.
 // A step is half a tile, 64 positions, so that each group has two S buffers: while it works on one, the tensor cores fill
 // the other. (With one buffer of 128 positions a group waited 1.6 us for its next scores after 1.0 us of work on them: P,
@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kPrefixTile = 128;  // positions of a tile
 constexpr int kGroupRows = 128;   // query rows of a softmax group
-constexpr int kPrefixThreads = 352;
+constexpr int kPrefixThreads = 384;
 constexpr int kStep = 64;         // positions of a step
 constexpr float kSlack = 8.0f;    // by how much a maximum may fall behind
 
@@ -185,42 +185,47 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const int units = a.kv_heads * a.row_tiles;
   const int first = blockIdx.x * p.run, last = min(first + p.run, units * p.tiles);
   bool dead = false;
-  if (warp == 8) {
+  if (warp == 8 || warp == 11) {
+    const bool is_v = warp == 11;
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    const CUtensorMap* map = is_v ? &value_map : &key_map;
+    const unsigned ring = smem_at + (is_v ? S::kOffV : S::kOffK);
     const int box_rows = 1 << p.rows_log, pages = kPrefixTile >> p.rows_log, blocks = a.head_dim == DT ? 1 : DT / 64;
     const int page_bytes = box_rows * 128 * (DT / 64);
+    const int outside = (int)(a.num_blocks * a.block_size);  // rows of zeros, which a weight of zero must meet
+    const bool leader = elect_one();
     const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
       const int pos = tile * kPrefixTile + lane * box_rows;
-      const int outside = (int)(a.num_blocks * a.block_size);  // zeros, which a weight of zero must meet
       if (lane >= pages || pos >= a.prefix) return outside;
       const int page = pos / a.block_size;
       const long long block = __ldg(a.tables + page);
       if (block < 0 || block >= a.num_blocks) return outside;
       return (int)(block * a.block_size + (pos - page * a.block_size));
     };
-    int row_now = page_of(first % p.tiles), in_piece = 0, uses0 = 0, uses1 = 0;
+    int unit = first / p.tiles, tile = first - unit * p.tiles;
+    int row_now = page_of(tile), in_piece = 0, uses0 = 0, uses1 = 0;
     for (int w = first; w < last; ++w) {
       // Alternate tiles of a piece have a stage each, that of their group, so that every group meets its stage's phases
       // one after the other.
-      const int n = w - first, kv_head = w / p.tiles / a.row_tiles;
-      if (w % p.tiles == 0) in_piece = 0;
-      const int stage = (alternate ? in_piece : n) & 1, use = stage == 0 ? uses0++ : uses1++;
+      const int stage = (alternate ? in_piece : w - first) & 1, use = stage == 0 ? uses0++ : uses1++;
+      const int kv_head = a.row_tiles == 1 ? unit : unit / a.row_tiles;
       ++in_piece;
-      const int row_next = page_of((w + 1) % p.tiles);
-      for (int is_v = 0; is_v < 2; ++is_v) {
-        uint64_t *full = (is_v ? v_full : k_full) + stage, *empty = (is_v ? v_empty : k_empty) + stage;
-        wait_or_give_up(empty, (use & 1) ^ 1, dead);
-        if (dead) break;
-        if (lane == 0) mbar_arrive_expect_tx(full, S::kTileBytes);
-        __syncwarp();
-        for (int i = lane; __any_sync(0xffffffffu, i < pages * blocks); i += 32) {
-          const int page = i % pages, block = i / pages;
-          const int row = __shfl_sync(0xffffffffu, row_now, page);
-          if (block < blocks)
-            tma_load4(smem_at + (is_v ? S::kOffV : S::kOffK) + stage * S::kTileBytes + page * page_bytes + block * (box_rows * 128),
-                      is_v ? &value_map : &key_map, block * 64, row, kv_head, full);
-        }
+      if (++tile == p.tiles) {
+        tile = in_piece = 0;
+        ++unit;
       }
+      const int row_next = page_of(tile);  // on its way while this tile's copies are issued
+      wait_or_give_up(&empty[stage], (use & 1) ^ 1, dead);
       if (dead) break;
+      if (leader) mbar_arrive_expect_tx(&full[stage], S::kTileBytes);
+      const unsigned at = ring + stage * S::kTileBytes;
+#pragma unroll 1
+      for (int page = 0; page < pages; ++page) {
+        const int row = __shfl_sync(0xffffffffu, row_now, page);
+        if (leader)
+          for (int block = 0; block < blocks; ++block)
+            tma_load4(at + page * page_bytes + block * (box_rows * 128), map, block * 64, row, kv_head, &full[stage]);
+      }
       row_now = row_next;
     }
   } else if (warp >= 9) {
@@ -303,31 +308,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const int kv_head = unit / a.row_tiles;
       const int row0 = (unit - kv_head * a.row_tiles) * p.unit_rows + (alternate ? 0 : g * kGroupRows);
       const bool any = !alternate || g < count;  // a piece of one tile has nothing for the second group
-      // The piece's queries, in the products' layout. All loads go out together.
-      constexpr int kChunks = DT / 8;
+      // The piece's queries, in the products' layout. The copies of all rows are under way together. (Loops here and below
+      // stay rolled up: each line of code that runs once costs its fetch, 14000 clocks in all for an unrolled form.)
       if (any) {
         const Row mine = row_of<true>(a, 0, kv_head, row0 + row);
         sync_warps(1 + g, kGroupRows);  // the last piece's rows have left these bytes, and their offsets are read
         row_offset[row] = mine.real ? mine.b * a.vq.batch + mine.t * a.vq.token + mine.head * a.vq.head : -1;
         sync_warps(1 + g, kGroupRows);
+        constexpr int kChunks = DT / 8;
         const int chunk = row % kChunks;
-        const T* q = (const T*)a.q + chunk * 8;
-        uint4 v[kChunks];
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          const long long off = row_offset[(i * kGroupRows + row) / kChunks];
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (off >= 0 && chunk * 8 < a.head_dim) v[i] = __ldg(reinterpret_cast<const uint4*>(q + off));
+        const unsigned q_to = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf;
+#pragma unroll 2
+        for (int r = row / kChunks; r < kGroupRows; r += kGroupRows / kChunks) {
+          const long long off = row_offset[r];
+          const bool fill = off >= 0 && chunk * 8 < a.head_dim;
+          copy16(q_to + r * 128 + (((chunk ^ r) & 7) << 4), (const T*)a.q + (fill ? off + chunk * 8 : 0), fill);
         }
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          const int r = (i * kGroupRows + row) / kChunks;
-          const unsigned at = smem_at + g * (kGroupRows * DT * 2) + (chunk >> 3) * S::kHalf + r * 128 + (((chunk ^ r) & 7) << 4);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
-                       : "memory");
-        }
-      }
-      if (any) {
+        copy_commit();
+        copy_wait<0>();
         fence_proxy_async();
         mbar_arrive(&q_full[g]);
       }
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           // The last step's product has reached O (the one before it had, or these scores would not be there).
           wait_or_give_up(&o_full[g * 2 + (buffer ^ 1)], (step - 1) >> 1 & 1, dead);
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DT; c += 32) {
             unsigned o[32];
             tmem_load32(o_at + c, o);
@@ -410,9 +408,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       constexpr int kCols = DT / 2, kParts = kCols / 4;  // columns at a time, 16-byte chunks of them
       const unsigned stage = smem_at + g * (kGroupRows * DT * 2) + (warp & 3) * (32 * kCols * 4);
       const int row_first = (warp & 3) * 32, rows = a.batch * a.rows - (row0 + row_first);
-#pragma unroll
+#pragma unroll 1
       for (int c0 = 0; c0 < DT; c0 += kCols) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kCols; c += 32) {
           unsigned o[32];
           tmem_load32(o_at + c0 + c, o);

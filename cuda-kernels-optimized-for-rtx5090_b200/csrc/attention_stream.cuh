@@ -94,7 +94,7 @@ template <typename T, int DT, int WR>
 __global__ void __launch_bounds__(32 * (kConsumers + 1))
     attend_stream(const Args a, int rows_log, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
   using S = Ring<DT, WR>;
-  constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages, kHalves = DT / 64;
+  constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages;
   constexpr int kAll = 32 * (kConsumers + 1);
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
