@@ -27,6 +27,10 @@ namespace {
 
 constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
+#ifndef CKB_PREFIX_SHARE
+#define CKB_PREFIX_SHARE 6
+#endif
+constexpr int kPrefixShare = CKB_PREFIX_SHARE;  // eighths of the SMs that the shared work takes
 constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -48,6 +52,7 @@ struct Args {
   int rows;        // tokens * group: query rows of a sequence and kv head
   int row_tiles;   // row tiles of a unit's rows
   float scale_log2;
+  bool beside;     // own work launched beside the shared work: see start_all
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   const unsigned smem_at = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, wk = warp / WR;
-  pdl_wait();
+  if (kShared || !a.beside) pdl_wait();
   pdl_trigger();
 
   // The axis of tiles.
@@ -298,6 +303,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   }
   const int first = (int)min((long long)blockIdx.x * run, (long long)all);
   const int last = min(first + run, all);
+  if (!kShared && a.beside && blockIdx.x == 0 && first >= last) pdl_wait();
   if (first >= last) return;
 
   // The cache row of position (tile, lane of the tile), or -1.
@@ -558,6 +564,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
     }
   }
   copy_wait<0>();
+  if (!kShared && a.beside && blockIdx.x == 0) pdl_wait();  // this grid ends after the shared work's
 }
 
 }  // namespace
@@ -724,7 +731,7 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
     h.unit_rows = i == 0 && rows * batch > kGroupRows ? 2 * kGroupRows : h.rows;
     h.slots = i == 0 ? 2 : 1;
     h.row_tiles = (int)((rows * batch + h.unit_rows - 1) / h.unit_rows);
-    const int tile = i == 0 ? kPrefixTile : kTile, at_once = i == 0 ? device_sm_count() : most;
+    const int tile = i == 0 ? kPrefixTile : kTile, at_once = i == 0 ? device_sm_count() * kPrefixShare / 8 : most;
     h.tiles = (int)((prefix + tile - 1) / tile);
     const long long all = (long long)h.tiles * kv_heads * h.row_tiles;
     if (all > INT_MAX / 2) return false;
@@ -851,8 +858,13 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
   // Two groups' O and S of 256 columns each do not fit TMEM: heads of more than 128 columns take attend_tiles.
   const bool tensor = maps.fit && dt <= 128;
   const auto& h = z.shared[tensor ? 0 : 1];
+  // The own work does not need the shared work's results, only the join does. So where both are there, it does not wait for
+  // it: the shared work's CTAs wait for what came before on the stream and then let the own work's start, on the SMs that
+  // they leave free and on theirs as they end; the own work's first CTA waits for the shared work before it ends, so that the
+  // join, which waits for the own work, follows both.
   cudaError_t err = cudaSuccess;
   Args s = a;
+  a.beside = a.prefix > 0;
   a.row_tiles = z.own_row_tiles;
   a.part = reinterpret_cast<float*>(work + z.off_own);
   a.ml = reinterpret_cast<float2*>(work + z.off_own_ml);

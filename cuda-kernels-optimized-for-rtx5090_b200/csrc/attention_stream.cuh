@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     tma_prefetch(&key_map);
     tma_prefetch(&value_map);
   }
-  pdl_wait();
+  if (!a.beside) pdl_wait();
   pdl_trigger();
   const int units = a.kv_heads * a.row_tiles;
   own_axis<kAll>(a, units, cum, lens, reinterpret_cast<int*>(ml_sh));  // its barriers order the mbarriers' set-up too
@@ -126,7 +126,11 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   }
   const int first = (int)min((long long)blockIdx.x * run, (long long)all);
   const int last = min(first + run, all);
-  if (first >= last) return;
+  // The first CTA, which always has a loading warp, ends after the shared work.
+  if (first >= last) {
+    if (a.beside && blockIdx.x == 0) pdl_wait();
+    return;
+  }
   Cursor at = axis_start(cum, a.batch, units, first);
   bool dead = false;
 
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
       axis_next(cum, a.batch, units, ahead);
       const int row_next = w + 1 < last ? page_of(ahead) : -1;  // behind this tile's copies
       wait_or_give_up(&empty[stage], (((w - first) / kStages) & 1) ^ 1, dead);
-      if (dead) return;
+      if (dead) break;
       const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));
       if (lane == 0) mbar_arrive_expect_tx(&full[stage], there * 2 * page_bytes);
       for (int i = lane; __any_sync(0xffffffffu, i < pages * blocks * 2); i += 32) {
@@ -180,6 +184,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     }
     copy_commit();
     copy_wait<0>();
+    if (a.beside && blockIdx.x == 0) pdl_wait();
     return;
   }
 
