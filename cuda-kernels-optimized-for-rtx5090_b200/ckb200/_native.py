@@ -84,9 +84,24 @@ def load(op):
     return lib
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t):
     """The current torch stream of t's device, as the cudaStream_t handle the C ABI takes."""
+    if _raw_stream is not None:  # the same handle without a Stream object around it (3 us of a call's host time)
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def call(fn, t, *args):
+    """fn(*args, stream): a library call on t's device and the current stream there. Raises by check()."""
+    index = t.device.index
+    if index == torch.cuda.current_device():  # the context manager alone takes 4 us
+        check(fn(*args, stream_of(t)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, stream_of(t)))
 
 
 def check(err):
@@ -97,10 +112,10 @@ def check(err):
 
 
 def require_cuda(op, *tensors):
+    dev = tensors[0].device
     for t in tensors:
         if not t.is_cuda:
             raise ValueError(f"{op}: tensors must be on a CUDA device (there is no CPU path), got {t.device}")
-    dev = tensors[0].device
     for t in tensors[1:]:
         if t.device != dev:
             raise ValueError(f"{op}: tensors on different devices: {dev} and {t.device}")

@@ -71,26 +71,24 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
         raise ValueError("attention: out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
     if batch == 0:
         return out
-    strides = [0 if n == 1 else st for n, st in zip(q.shape[:3], q.stride()[:3])]
-    if q.stride(3) != 1 or q.data_ptr() % 16 or any(st % 8 for st in strides):
+    st_b, st_t, st_h, st_d = q.stride()
+    st_b, st_t, st_h = 0 if batch == 1 else st_b, 0 if tokens == 1 else st_t, 0 if q_heads == 1 else st_h
+    if st_d != 1 or st_b % 8 or st_t % 8 or st_h % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-        strides = q.stride()[:3]
+        st_b, st_t, st_h, _ = q.stride()
     tables, lens = block_tables.contiguous(), seq_lens.contiguous()
     num_blocks, block_size, kv_heads, _ = key_cache.shape
+    width = tables.shape[1]
     lib = _native.load("attention")
-    with torch.cuda.device(q.device):
-        sizes = (batch, tokens, q_heads, kv_heads, head_dim, block_size, tables.shape[1], shared_prefix)
-        need = lib.ckb_attention_workspace(*sizes)
-        if need < 0:
-            raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
-                             f"block_tables {tuple(tables.shape)}")
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        err = lib.ckb_attention_paged_launch(q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), tables.data_ptr(),
-                                             lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES(*strides),
-                                             batch, tokens, q_heads, kv_heads, head_dim, num_blocks, block_size,
-                                             tables.shape[1], shared_prefix, scale, _DTYPES[q.dtype],
-                                             _native.stream_of(q))
-    _native.check(err)
+    need = lib.ckb_attention_workspace(batch, tokens, q_heads, kv_heads, head_dim, block_size, width, shared_prefix)
+    if need < 0:
+        raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
+                         f"block_tables {tuple(tables.shape)}")
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _native.call(lib.ckb_attention_paged_launch, q, q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                 tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES(st_b, st_t, st_h),
+                 batch, tokens, q_heads, kv_heads, head_dim, num_blocks, block_size, width, shared_prefix, scale,
+                 _DTYPES[q.dtype])
     return out
 
 

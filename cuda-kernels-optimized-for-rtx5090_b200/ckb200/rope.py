@@ -159,13 +159,15 @@ _STRIDES = ctypes.c_longlong * 15
 
 def _strides(t):
     """The batch, token and head strides of a [B, S, heads, D] view (0 for a dim of size 1, whose stride is any)."""
-    return [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()[:3])]
+    b, s, h, _ = t.shape
+    st_b, st_s, st_h, _ = t.stride()
+    return 0 if b == 1 else st_b, 0 if s == 1 else st_s, 0 if h == 1 else st_h
 
 
 def _strided(t, name=None):
     """t where its last dim is contiguous (a view of a fused projection is), else a contiguous copy; with a name (of an
     in-place output) a tensor that cannot be written through its view raises."""
-    unit = t.shape[3] == 1 or t.stride(3) == 1
+    unit = t.stride(3) == 1 or t.shape[3] == 1
     if name is None:
         return t if unit else t.contiguous()
     if not unit or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
@@ -179,30 +181,37 @@ def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches,
     problem = _problem(q, k, cos, sin, position_ids)
     if problem:
         raise ValueError(f"rope candidate: {problem}")
-    q_heads, kv_heads, head_dim = q.shape[2], k.shape[2], q.shape[3]
+    batch, seq, q_heads, head_dim = q.shape
+    k_shape = k.shape
+    kv_heads = k_shape[2]
     if q_heads < 1 or kv_heads < 1 or head_dim < 2:
         raise ValueError(f"rope candidate: shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype not in _CACHE or w.dtype != q_weight.dtype or tuple(w.shape) != (head_dim,):
-            raise ValueError(f"rope candidate: {name} must be [{head_dim}] of fp32, bf16 or fp16 (both the same), got "
-                             f"{w.dtype} {tuple(w.shape)}")
-    if cos is not None and cos.shape[0] < 1:
-        raise ValueError("rope candidate: the cos/sin cache has no rows")
-    tensors = [q, k, position_ids, q_weight, k_weight] + ([] if cos is None else [cos, sin])
-    slots = None
+    w_dtype = _CACHE.get(q_weight.dtype)
+    if w_dtype is None or k_weight.dtype != q_weight.dtype or q_weight.shape != (head_dim,) or \
+            k_weight.shape != (head_dim,):
+        raise ValueError(f"rope candidate: q_weight and k_weight must be [{head_dim}] of fp32, bf16 or fp16 (both the same), "
+                         f"got {q_weight.dtype} {tuple(q_weight.shape)} and {k_weight.dtype} {tuple(k_weight.shape)}")
+    tensors = [q, k, position_ids, q_weight, k_weight]
+    cos_at = sin_at = freqs_at = v_at = slots_at = key_at = value_at = None
+    positions = cache_slots = cache_dtype = 0
+    if cos is not None:
+        positions = cos.shape[0]
+        if positions < 1:
+            raise ValueError("rope candidate: the cos/sin cache has no rows")
+        tensors += cos, sin
     if caches is not None:
-        if v.shape != k.shape or v.dtype != k.dtype:
+        if v.shape != k_shape or v.dtype != k.dtype:
             raise ValueError(f"rope candidate: v {v.dtype} {tuple(v.shape)} must match k {k.dtype} {tuple(k.shape)}")
         for name, c in zip(("key_cache", "value_cache"), caches):
-            if c.dtype != q.dtype or c.dim() != 4 or tuple(c.shape[2:]) != tuple(k.shape[2:]) or not c.is_contiguous():
+            if c.dtype != q.dtype or c.dim() != 4 or c.shape[2:] != k_shape[2:] or not c.is_contiguous():
                 raise ValueError(f"rope candidate: {name} must be a contiguous [blocks, block_size, {kv_heads}, "
                                  f"{head_dim}] tensor of {q.dtype}, got {c.dtype} {tuple(c.shape)}")
         if caches[0].shape != caches[1].shape:
             raise ValueError(f"rope candidate: key_cache {tuple(caches[0].shape)} and value_cache "
                              f"{tuple(caches[1].shape)} differ")
-        if slot_mapping.dtype != torch.int64 or tuple(slot_mapping.shape) != tuple(position_ids.shape):
+        if slot_mapping.dtype != torch.int64 or slot_mapping.shape != position_ids.shape:
             raise ValueError(f"rope candidate: slot_mapping must be int64 {tuple(position_ids.shape)}")
-        tensors += [v, *caches, slot_mapping]
+        tensors += v, slot_mapping, *caches
     _native.require_cuda("rope", *tensors)
     if inplace:
         q_out, k_out = _strided(q, "q"), (_strided(k, "k") if write_k else None)
@@ -211,39 +220,30 @@ def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches,
         q, k = _strided(q), _strided(k)
         if out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if write_k else None
+            k_out = torch.empty(k_shape, dtype=q.dtype, device=q.device) if write_k else None
         else:
             q_out, k_out = out
             for o, t in ((q_out, q), (k_out, k)):
                 if o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous() or o.device != t.device:
                     raise ValueError("rope candidate: out must be contiguous tensors of q's and k's shapes, dtype "
                                      "and device")
+    ids, q_weight, k_weight = position_ids.contiguous(), q_weight.contiguous(), k_weight.contiguous()
+    if cos is None:
+        freqs_at = inv_freq(theta, head_dim, q.device).data_ptr()
+    else:
+        cos, sin = cos.contiguous(), sin.contiguous()
+        cos_at, sin_at, cache_dtype = cos.data_ptr(), sin.data_ptr(), _CACHE[cos.dtype]
+    none = (0, 0, 0)
     if caches is not None:
         v, slots = _strided(v), slot_mapping.contiguous()
-    ids, q_weight, k_weight = position_ids.contiguous(), q_weight.contiguous(), k_weight.contiguous()
-    strides = _STRIDES(*_strides(q), *_strides(k), *(_strides(v) if caches is not None else (0, 0, 0)), *_strides(q_out),
-                       *(_strides(k_out) if k_out is not None else (0, 0, 0)))
-    batch, seq = ids.shape
-    lib = _native.load("rope")
-    with torch.cuda.device(q.device):
-        freqs = None
-        if cos is None:
-            freqs = inv_freq(theta, head_dim, q.device)
-        else:
-            cos, sin = cos.contiguous(), sin.contiguous()
-
-        def ptr(t):
-            return None if t is None else t.data_ptr()
-
-        key_cache, value_cache = caches if caches is not None else (None, None)
-        err = lib.ckb_rope_qk_norm_launch(ptr(q), ptr(k), ptr(v if caches is not None else None), ptr(q_weight),
-                                          ptr(k_weight), ptr(cos), ptr(sin), ptr(freqs), ptr(ids), ptr(slots),
-                                          ptr(q_out), ptr(k_out), ptr(key_cache), ptr(value_cache), strides,
-                                          0 if cos is None else cos.shape[0],
-                                          0 if key_cache is None else key_cache.shape[0] * key_cache.shape[1], batch,
-                                          seq, q_heads, kv_heads, head_dim, _QK[q.dtype], _CACHE[q_weight.dtype],
-                                          0 if cos is None else _CACHE[cos.dtype], float(eps), _native.stream_of(q))
-    _native.check(err)
+        v_at, slots_at, key_at, value_at = v.data_ptr(), slots.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr()
+        cache_slots = caches[0].shape[0] * caches[0].shape[1]
+    strides = _STRIDES(*_strides(q), *_strides(k), *(none if caches is None else _strides(v)), *_strides(q_out),
+                       *(none if k_out is None else _strides(k_out)))
+    _native.call(_native.load("rope").ckb_rope_qk_norm_launch, q, q.data_ptr(), k.data_ptr(), v_at, q_weight.data_ptr(),
+                 k_weight.data_ptr(), cos_at, sin_at, freqs_at, ids.data_ptr(), slots_at, q_out.data_ptr(),
+                 None if k_out is None else k_out.data_ptr(), key_at, value_at, strides, positions, cache_slots, batch,
+                 seq, q_heads, kv_heads, head_dim, _QK[q.dtype], w_dtype, cache_dtype, eps)
     return q_out, k_out
 
 
@@ -254,7 +254,8 @@ def qk_norm_rope(q, k, position_ids, q_weight, k_weight, cos=None, sin=None, the
     k_weight ([D], fp32, bf16 or fp16), fp32 math with one rounding at the end. q and k may be views of a fused
     projection (any strides, the last dim contiguous). cos / sin [max_position, D] picked by position_ids (an id
     outside takes the nearest row), or theta; inplace and out as in rope(). Returns (q_out, k_out)."""
-    return _qk_norm(q, k, None, position_ids, q_weight, k_weight, cos, sin, theta, None, None, eps, inplace, True, out)
+    return _qk_norm(q, k, None, position_ids, q_weight, k_weight, cos, sin, theta, None, None, float(eps), inplace, True,
+                    out)
 
 
 def qk_norm_rope_kv_cache(q, k, v, position_ids, q_weight, k_weight, cos, sin, key_cache, value_cache, slot_mapping,
@@ -264,4 +265,4 @@ def qk_norm_rope_kv_cache(q, k, v, position_ids, q_weight, k_weight, cos, sin, k
     Hkv, D], as rope_kv_cache does (a slot outside the caches, a padding token's, is not written). q, k and v may be
     views of a fused projection; in place writes through them. Returns (q_out, k_out or None)."""
     return _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, (key_cache, value_cache), slot_mapping,
-                    eps, inplace, write_k, None)
+                    float(eps), inplace, write_k, None)

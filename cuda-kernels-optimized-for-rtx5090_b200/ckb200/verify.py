@@ -32,6 +32,14 @@ def _problem(target, tokens, uniforms, draft, counts):
     return None
 
 
+def _strided(t):
+    """t (copied where its last dim is not contiguous) and its first two strides, 0 for a dim of size 1."""
+    if t.stride(2) != 1 and t.shape[2] != 1:
+        t = t.contiguous()
+    batch, row, _ = t.stride()
+    return t, 0 if t.shape[0] == 1 else batch, 0 if t.shape[1] == 1 else row
+
+
 def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, num_drafts=None, out=None):
     """Checks drafted tokens: (tokens [B, K + 1], accepted [B]), int64. Row b of tokens holds the accepted drafted tokens,
     then the newly drawn one, then -1; accepted[b] counts the first.
@@ -58,22 +66,15 @@ def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, num_dr
             if tuple(t.shape) != shape or t.dtype != torch.int64 or not t.is_contiguous() or \
                     t.device != target_probs.device:
                 raise ValueError("verify: out must be contiguous int64 tensors [B, K + 1] and [B] on target_probs' device")
-    target, draft = (t if t is None or vocab == 1 or t.stride(2) == 1 else t.contiguous()
-                     for t in (target_probs, draft_probs))
+    target, target_batch, target_row = _strided(target_probs)
+    draft, draft_batch, draft_row = (None, 0, 0) if draft_probs is None else _strided(draft_probs)
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
     counts = None if num_drafts is None else num_drafts.contiguous()
-
-    def strides(t):
-        return (0, 0) if t is None else tuple(0 if t.shape[i] == 1 else t.stride(i) for i in (0, 1))
-
-    lib = _native.load("verify")
-    with torch.cuda.device(target.device):
-        err = lib.ckb_verify_launch(target.data_ptr(), None if draft is None else draft.data_ptr(),
-                                    draft_tokens.data_ptr(), None if counts is None else counts.data_ptr(),
-                                    uniforms.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), *strides(target),
-                                    *strides(draft), batch, rows - 1, vocab, _DTYPES[target.dtype],
-                                    _native.stream_of(target))
-    _native.check(err)
+    _native.call(_native.load("verify").ckb_verify_launch, target, target.data_ptr(),
+                 None if draft is None else draft.data_ptr(), draft_tokens.data_ptr(),
+                 None if counts is None else counts.data_ptr(), uniforms.data_ptr(), tokens.data_ptr(),
+                 accepted.data_ptr(), target_batch, target_row, draft_batch, draft_row, batch, rows - 1, vocab,
+                 _DTYPES[target.dtype])
     return tokens, accepted
 
 

@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
+constexpr int kMaxShared = 232448;  // bytes of shared memory that a CTA can have
 #ifndef CKB_PREFIX_SHARE
 #define CKB_PREFIX_SHARE 6
 #endif
@@ -750,12 +751,25 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
   return true;
 }
 
+// Lets a kernel have all of an SM's shared memory, once for each device (up to 64; a call takes a microsecond).
+template <typename K>
+cudaError_t open_shared_memory(K* kernel, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+  if (err == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return err;
+}
+
 template <typename T, int DT, int WR, bool kShared>
 cudaError_t start(const Args& a, int ctas, cudaStream_t stream) {
   using S = Shape<T, DT, WR, kShared>;
   const int bytes = S::bytes(a.batch);
-  const cudaError_t err = cudaFuncSetAttribute(attend_tiles<T, DT, WR, kShared>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t err = open_shared_memory(attend_tiles<T, DT, WR, kShared>, done);
   if (err != cudaSuccess) return err;
   return launch_pdl(attend_tiles<T, DT, WR, kShared>, dim3(ctas), dim3(kThreads), bytes, stream, a);
 }
@@ -818,8 +832,8 @@ Maps maps_of(const Args& a, int rows_log) {
 template <typename T, int DT, int WR>
 cudaError_t start_stream(const Args& a, int ctas, const Maps& maps, cudaStream_t stream) {
   const int bytes = Ring<DT, WR>::bytes(a.batch);
-  const cudaError_t err =
-      cudaFuncSetAttribute(attend_stream<T, DT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t err = open_shared_memory(attend_stream<T, DT, WR>, done);
   if (err != cudaSuccess) return err;
   return launch_pdl(attend_stream<T, DT, WR>, dim3(ctas), dim3(32 * (kConsumers + 1)), bytes, stream, a, maps.rows_log,
                     maps.keys, maps.values);
@@ -843,7 +857,8 @@ cudaError_t start_prefix(const Args& a, const Sizes& z, cudaStream_t stream) {
   if (!maps.fit) return cudaErrorInvalidValue;
   const auto& h = z.shared[0];
   const int bytes = PrefixShape<DT>::kBytes;
-  const cudaError_t err = cudaFuncSetAttribute(attend_prefix<T, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t err = open_shared_memory(attend_prefix<T, DT>, done);
   if (err != cudaSuccess) return err;
   const PrefixArgs p{a, h.tiles, h.run, h.unit_rows, maps.rows_log};
   return launch_pdl(attend_prefix<T, DT>, dim3(h.ctas), dim3(kPrefixThreads), bytes, stream, p, maps.keys, maps.values);

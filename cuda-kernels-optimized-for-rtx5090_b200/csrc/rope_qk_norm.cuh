@@ -10,8 +10,12 @@
 //
 // HBM bound: each element is read once and written once; cos/sin rows and weights are L2/L1 hits. A head belongs to a
 // group of G = 2^n >= D / 16 lanes of one warp, lane c holding the pairs 8c..8c+7 (both halves), so the sum of squares
-// is a G-wide shuffle and nothing goes through shared memory. As in rope_tokens a thread keeps up to kNormHeads heads'
-// loads in flight and uses one fetch of its cos/sin values for all of them.
+// is a G-wide shuffle and nothing goes through shared memory. A group takes up to kNormGroup heads of ONE kind (query, key
+// or value) of a token, so it has one weight, and w cos and w sin are multiplied once for all its heads; the loads of
+// kNormHeads heads are in flight all along, each replaced as soon as its head is worked on. Arithmetic is in pairs (packed
+// fp32). 8 x 4096 tokens of 32 + 8 heads x 128 in bf16 take 129 us, 5.3 TB/s or 0.82 of the measured copy bandwidth. (Groups
+// of mixed kinds with the weight and the angles apart took 167 us; lanes that left early, which makes every shuffle of the
+// others ask who is there, 162 us.)
 #pragma once
 
 namespace ckb {
@@ -57,116 +61,124 @@ __device__ __forceinline__ long long cache_slot(const NormArgs& a, unsigned toke
   return slot < a.cache_slots ? slot : -1;
 }
 
-#ifndef CKB_QK_NORM_HEADS
-#define CKB_QK_NORM_HEADS 5
-#endif
-constexpr int kNormHeads = CKB_QK_NORM_HEADS;
+// Measured at 8 x 4096 tokens of 32 + 8 heads x 128 in bf16: 4 heads in flight of groups of 8 on two CTAs an SM (104 registers)
+// 129 us; 2 heads 140 us; 5 to 8 heads 148 us and more; groups of 4 153 us, of 16 133 us; three CTAs, which spill, 190 us.
+constexpr int kNormHeads = 4;  // heads of a group whose loads are in flight
+constexpr int kNormGroup = 8;  // heads of a group at most
 
-// Block (G, R, Z): lane threadIdx.x of heads threadIdx.y, + R, + 2R, ... of token blockIdx.x * Z + threadIdx.z. Heads
-// run over q, then k, then (with a cache) v. Every thread takes every round, so a group's shuffles always meet.
+__device__ __forceinline__ float2 as2(const float (&f)[8], int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// Groups of G lanes lie one after the other through the grid: group_count of a token (its queries, then keys, then, with a
+// cache, values, `per` heads each), then the next token's. No lane leaves early, so the shuffles take the whole warp.
 template <typename T, bool kCache>
-__global__ void __launch_bounds__(256) qk_norm_rope_tokens(const NormArgs a) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_tokens(const NormArgs a, int lanes_log, int per,
+                                                                               int group_count) {
   pdl_wait();
   pdl_trigger();
-  const unsigned token = blockIdx.x * blockDim.z + threadIdx.z;
+  const int G = 1 << lanes_log;
+  const unsigned id = blockIdx.x * (256u >> lanes_log) + (threadIdx.x >> lanes_log);
+  const unsigned token = id / group_count;
+  int group = id - token * group_count;
   const int half = a.head_dim >> 1;
-  const int c = threadIdx.x * 8;
+  const int c = (threadIdx.x & (G - 1)) * 8;
+  const int q_groups = (a.q_heads + per - 1) / per, k_groups = (a.kv_heads + per - 1) / per;
+  const bool is_q = group < q_groups, is_v = group >= q_groups + k_groups;
+  group -= is_q ? 0 : is_v ? q_groups + k_groups : q_groups;
+  const int h0 = group * per;
   const bool active = token < a.tokens && c < half;
+  const int count = active ? min(per, (is_q ? a.q_heads : a.kv_heads) - h0) : 0;
   const unsigned b = token / a.seq, s = token - b * a.seq;
-  const int R = blockDim.y;
-  const int qk_heads = a.q_heads + a.kv_heads;
-  const int heads = qk_heads + (a.slots != nullptr ? a.kv_heads : 0);
-  const int G = blockDim.x;
-  const unsigned lane = (threadIdx.x + G * (threadIdx.y + R * threadIdx.z)) & 31u;
-  const unsigned group_mask = (G == 32 ? 0xffffffffu : ((1u << G) - 1u)) << (lane & ~(G - 1u));
-  const T* q = (const T*)a.q + b * a.vq.batch + s * a.vq.token + c;
-  const T* k = (const T*)a.k + b * a.vk.batch + s * a.vk.token + c;
-  const T* v = (const T*)a.v + b * a.vv.batch + s * a.vv.token + c;
+  const long long in_head = is_q ? a.vq.head : is_v ? a.vv.head : a.vk.head;
+  const T* x = (const T*)(is_q ? a.q : is_v ? a.v : a.k) + h0 * in_head + c +
+               b * (is_q ? a.vq.batch : is_v ? a.vv.batch : a.vk.batch) +
+               s * (is_q ? a.vq.token : is_v ? a.vv.token : a.vk.token);
 
   const T tag{};  // selects the overloads of unpack16 / pack16
-  float c1[8], s1[8], c2[8], s2[8];
-  long long slot = -1;
-  for (int h0 = 0; h0 < heads; h0 += kNormHeads * R) {
-    uint4 ra[kNormHeads], rb[kNormHeads];
-#pragma unroll
-    for (int j = 0; j < kNormHeads; ++j) {  // every load of the round before any use
-      const int h = h0 + threadIdx.y + j * R;
-      const T* p = h < a.q_heads ? q + h * a.vq.head
-                   : h < qk_heads ? k + (h - a.q_heads) * a.vk.head
-                                  : v + (h - qk_heads) * a.vv.head;
-      if (active && h < heads) {
-        ra[j] = ld_inplace(p);
-        rb[j] = ld_inplace(p + half);
-      } else {
-        ra[j] = rb[j] = make_uint4(0u, 0u, 0u, 0u);
-      }
+  uint4 ra[kNormHeads], rb[kNormHeads];
+  const auto fetch = [&](int j, int h) {
+    ra[j] = rb[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (h < count) {
+      ra[j] = ld_inplace(x + h * in_head);
+      rb[j] = ld_inplace(x + h * in_head + half);
     }
-    if (h0 == 0 && active) {  // behind the first round's loads
-      const long long pos = __ldg(a.ids + token);
-      slot = cache_slot(a, token);
-      if constexpr (kCache) {
-        const long long row = cos_row(pos, a.positions) * a.head_dim + c;
-        ld8_any(a.cos_rows, a.cache_dtype, row, c1);
-        ld8_any(a.sin_rows, a.cache_dtype, row, s1);
-        ld8_any(a.cos_rows, a.cache_dtype, row + half, c2);
-        ld8_any(a.sin_rows, a.cache_dtype, row + half, s2);
-      } else {
-        const float p = (float)pos;
+  };
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sincosf(p * __ldg(a.inv_freq + c + e), &s1[e], &c1[e]);
-          c2[e] = c1[e];
-          s2[e] = s1[e];
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kNormHeads; ++j) {
-      const int h = h0 + threadIdx.y + j * R;
-      float x[8], z[8];
-      unpack16(ra[j], x, &tag);
-      unpack16(rb[j], z, &tag);
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], fmaf(z[e], z[e], ss));
-      for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(group_mask, ss, o);
-      if (!active || h >= heads) continue;
-      if (h >= qk_heads) {  // v: as it is, into its cache row
-        if (slot >= 0) {
-          T* dst = (T*)a.value_cache + (slot * a.kv_heads + (h - qk_heads)) * a.head_dim + c;
-          st_stream(dst, ra[j]);
-          st_stream(dst + half, rb[j]);
-        }
-        continue;
-      }
-      const float inv = rsqrtf(ss / (float)a.head_dim + a.eps);
-      const bool is_q = h < a.q_heads;
-      float w1[8], w2[8];
-      ld8_any(is_q ? a.q_weight : a.k_weight, a.w_dtype, c, w1);
-      ld8_any(is_q ? a.q_weight : a.k_weight, a.w_dtype, c + half, w2);
+  for (int j = 0; j < kNormHeads; ++j) fetch(j, j);  // before the angles and weights
+  const long long slot = is_q || token >= a.tokens ? -1 : cache_slot(a, token);
+  const long long out_head = is_q ? a.vq_out.head : a.vk_out.head;
+  T* out = (T*)(is_q ? a.q_out : is_v ? nullptr : a.k_out);
+  if (out != nullptr)
+    out += h0 * out_head + c + b * (is_q ? a.vq_out.batch : a.vk_out.batch) + s * (is_q ? a.vq_out.token : a.vk_out.token);
+  T* cache = slot < 0 ? nullptr : (T*)(is_v ? a.value_cache : a.key_cache) + (slot * a.kv_heads + h0) * a.head_dim + c;
+  // out_lo = x_lo inv (w_lo cos_lo) - x_hi inv (w_hi sin_lo), out_hi = x_hi inv (w_hi cos_hi) + x_lo inv (w_lo sin_hi)
+  float2 lo_lo[4], lo_hi[4], hi_hi[4], hi_lo[4];
+  if (active && !is_v) {
+    const long long pos = __ldg(a.ids + token);
+    float w1[8], w2[8], c1[8], s1[8], c2[8], s2[8];
+    const void* w = is_q ? a.q_weight : a.k_weight;
+    ld8_any(w, a.w_dtype, c, w1);
+    ld8_any(w, a.w_dtype, c + half, w2);
+    if constexpr (kCache) {
+      const long long row = cos_row(pos, a.positions) * a.head_dim + c;
+      ld8_any(a.cos_rows, a.cache_dtype, row, c1);
+      ld8_any(a.sin_rows, a.cache_dtype, row, s1);
+      ld8_any(a.cos_rows, a.cache_dtype, row + half, c2);
+      ld8_any(a.sin_rows, a.cache_dtype, row + half, s2);
+    } else {
+      const float p = (float)pos;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float lo = x[e] * inv * w1[e], hi = z[e] * inv * w2[e];
-        x[e] = lo * c1[e] - hi * s1[e];
-        z[e] = hi * c2[e] + lo * s2[e];
+        sincosf(p * __ldg(a.inv_freq + c + e), &s1[e], &c1[e]);
+        c2[e] = c1[e];
+        s2[e] = s1[e];
       }
-      const uint4 px = pack16(x, &tag), pz = pack16(z, &tag);
-      if (is_q) {
-        T* dst = (T*)a.q_out + b * a.vq_out.batch + s * a.vq_out.token + h * a.vq_out.head + c;
-        st_stream(dst, px);
-        st_stream(dst + half, pz);
-        continue;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo_lo[e] = __fmul2_rn(as2(w1, e), as2(c1, e));
+      lo_hi[e] = __fmul2_rn(as2(w2, e), make_float2(-s1[2 * e], -s1[2 * e + 1]));
+      hi_hi[e] = __fmul2_rn(as2(w2, e), as2(c2, e));
+      hi_lo[e] = __fmul2_rn(as2(w1, e), as2(s2, e));
+    }
+  }
+  for (int first = 0; first < per; first += kNormHeads) {
+#pragma unroll
+    for (int j = 0; j < kNormHeads; ++j) {
+      const int h = first + j;
+      float f[8], g[8];
+      unpack16(ra[j], f, &tag);
+      unpack16(rb[j], g, &tag);
+      uint4 px = ra[j], pz = rb[j];
+      fetch(j, h + kNormHeads);
+      float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = __ffma2_rn(as2(f, e), as2(f, e), __ffma2_rn(as2(g, e), as2(g, e), sum));
+      float ss = sum.x + sum.y;
+      for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (h >= count) continue;
+      if (!is_v) {  // a value goes to its cache row as it is
+        const float2 inv = twice(rsqrtf(ss / (float)a.head_dim + a.eps));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 lo = __fmul2_rn(as2(f, e), inv), hi = __fmul2_rn(as2(g, e), inv);
+          const float2 u = __ffma2_rn(lo, lo_lo[e], __fmul2_rn(hi, lo_hi[e]));
+          const float2 v = __ffma2_rn(hi, hi_hi[e], __fmul2_rn(lo, hi_lo[e]));
+          f[2 * e] = u.x;
+          f[2 * e + 1] = u.y;
+          g[2 * e] = v.x;
+          g[2 * e + 1] = v.y;
+        }
+        px = pack16(f, &tag);
+        pz = pack16(g, &tag);
       }
-      const int hk = h - a.q_heads;
-      if (a.k_out != nullptr) {
-        T* dst = (T*)a.k_out + b * a.vk_out.batch + s * a.vk_out.token + hk * a.vk_out.head + c;
-        st_stream(dst, px);
-        st_stream(dst + half, pz);
+      if (out != nullptr) {
+        st_stream(out + h * out_head, px);
+        st_stream(out + h * out_head + half, pz);
       }
-      if (slot >= 0) {
-        T* dst = (T*)a.key_cache + (slot * a.kv_heads + hk) * a.head_dim + c;
-        st_stream(dst, px);
-        st_stream(dst + half, pz);
+      if (cache != nullptr) {
+        st_stream(cache + h * a.head_dim, px);
+        st_stream(cache + h * a.head_dim + half, pz);
       }
     }
   }
@@ -251,18 +263,20 @@ int start_qk_norm(const NormArgs& a, cudaStream_t stream) {
                    aligned16(a.q_weight) && aligned16(a.k_weight) &&
                    (kCache ? aligned16(a.cos_rows) && aligned16(a.sin_rows) : aligned16(a.inv_freq));
   if (vec) {
-    int lanes = 1;
-    while (lanes * 16 < a.head_dim) lanes *= 2;
-    const int most = 256 / lanes;  // groups of a block
-    // Heads per thread: kNormHeads where that still leaves two blocks for each SM, else fewer.
-    int per = kNormHeads;
-    while (per > 1 && (long long)a.tokens * ((heads + per - 1) / per) < 2LL * device_sm_count() * most) --per;
-    int r = (heads + per - 1) / per;
-    if (r > most) r = most;
-    int z = most / r;
-    if (z > 64) z = 64;
-    const unsigned grid = (a.tokens + z - 1) / z;
-    launch_pdl(qk_norm_rope_tokens<T, kCache>, dim3(grid), dim3(lanes, r, z), 0, stream, a);
+    int lanes_log = 0;
+    while (16 << lanes_log < a.head_dim) ++lanes_log;
+    const int most = 256 >> lanes_log;  // groups of a block
+    // Heads per group: the most that still leaves two blocks for each SM.
+    int per = kNormGroup, groups = 0;
+    while (true) {
+      groups = (a.q_heads + per - 1) / per + (a.slots != nullptr ? 2 : 1) * ((a.kv_heads + per - 1) / per);
+      if (per == 1 || (long long)a.tokens * groups >= 2LL * device_sm_count() * most) break;
+      per /= 2;
+    }
+    const long long all = (long long)a.tokens * groups;
+    if (all > UINT_MAX - 256) return -1;
+    launch_pdl(qk_norm_rope_tokens<T, kCache>, dim3((unsigned)((all + most - 1) / most)), dim3(256), 0, stream, a, lanes_log,
+               per, groups);
   } else {
     launch_pdl(qk_norm_rope_scalar<T, kCache>, dim3(a.tokens), dim3(32, heads < 16 ? heads : 16), 0, stream, a);
   }
