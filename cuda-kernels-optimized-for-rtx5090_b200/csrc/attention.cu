@@ -49,6 +49,7 @@ struct Args {
   View3 vq;
   long long num_blocks;
   int batch, tokens, q_heads, kv_heads, group, head_dim, block_size, table_width;
+  int block_log;   // log2 of block_size, or -1
   int prefix;      // positions of the shared prefix
   int rows;        // tokens * group: query rows of a sequence and kv head
   int row_tiles;   // row tiles of a unit's rows
@@ -599,9 +600,9 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kWarps;
-  const long long row = (long long)blockIdx.x * (8 / kWarps) + warp / kWarps;
-  if (row >= (long long)a.batch * a.tokens * a.q_heads) return;
-  const int head = (int)(row % a.q_heads), t = (int)(row / a.q_heads % a.tokens), b = (int)(row / a.q_heads / a.tokens);
+  const int b = blockIdx.y, row = blockIdx.x * (8 / kWarps) + warp / kWarps;  // row of the sequence
+  if (row >= a.tokens * a.q_heads) return;
+  const int t = row / a.q_heads, head = row - t * a.q_heads;
   const int kv_head = head / a.group, in = t * a.group + (head - kv_head * a.group);
 
   // Own pieces: slots own_slot, own_slot + 1, ...; shared ones the same.
@@ -631,42 +632,41 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
       shared_step = a.shared_rows;
     }
   }
-  const auto at = [&](int i) { return i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * shared_step; };
   const int pieces = own + shared;
-  const auto ml_of = [&](int i) { return (i < own ? a.own_ml : a.shared_ml)[at(i)]; };
-  float top = -INFINITY, sum = 0.0f;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, ml_of(i).x);
-  top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  for (int i = lane; i < pieces; i += 32) {
-    const float2 v = ml_of(i);
-    sum += v.y * exp2_fast(v.x - ref);
-  }
-  sum = warp_sum(sum);
   const bool some = len - a.tokens + t + 1 > 0;
-  const float inv = 1.0f / sum;
-  T* out = (T*)a.out + row * a.head_dim;
+  T* out = (T*)a.out + ((long long)b * a.tokens * a.q_heads + row) * a.head_dim;
   __shared__ float4 partial[kWarps > 1 ? 8 : 1][32];
+  __shared__ float2 partial_ml[8];
   for (int c0 = 0; c0 < a.head_dim; c0 += 128) {
     const int c = c0 + lane * 4;
     const bool inside = some && c < a.head_dim;
+    float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int i0 = part; i0 < pieces; i0 += kAhead * kWarps) {
       float4 v[kAhead];
-      float w[kAhead];
+      float2 ml[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
+      for (int k = 0; k < kAhead; ++k) {  // statistics and sums together
         const int i = i0 + k * kWarps;
         v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        w[k] = -INFINITY;
+        ml[k] = make_float2(-INFINITY, 0.0f);
         if (i < pieces) {
-          w[k] = ml_of(i).x;
-          if (inside) v[k] = *reinterpret_cast<const float4*>((i < own ? a.own_part : a.shared_part) + at(i) * a.head_dim + c);
+          const long long w = i < own ? own_at + (long long)i * a.own_rows : shared_at + (long long)(i - own) * shared_step;
+          ml[k] = (i < own ? a.own_ml : a.shared_ml)[w];
+          if (inside) v[k] = *reinterpret_cast<const float4*>((i < own ? a.own_part : a.shared_part) + w * a.head_dim + c);
         }
       }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) top = fmaxf(top, ml[k].x);
+      const float ref = top == -INFINITY ? 0.0f : top, down = exp2_fast(m - ref);
+      m = top;
+      l *= down;
+      acc = make_float4(acc.x * down, acc.y * down, acc.z * down, acc.w * down);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const float x = exp2_fast(w[k] - ref);
+        const float x = exp2_fast(ml[k].x - ref);
+        l = fmaf(x, ml[k].y, l);
         acc.x = fmaf(x, v[k].x, acc.x);
         acc.y = fmaf(x, v[k].y, acc.y);
         acc.z = fmaf(x, v[k].z, acc.z);
@@ -675,17 +675,27 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
     }
     if (kWarps > 1) {
       partial[warp][lane] = acc;
+      if (lane == 0) partial_ml[warp] = make_float2(m, l);
       __syncthreads();  // a block has one row then
       if (part == 0) {
+        float top = m;
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) {
+        for (int k = 1; k < kWarps; ++k) top = fmaxf(top, partial_ml[k].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        l = 0.0f;
+        acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
           const float4 v = partial[k][lane];
-          acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+          const float x = exp2_fast(partial_ml[k].x - ref);
+          l = fmaf(x, partial_ml[k].y, l);
+          acc = make_float4(fmaf(x, v.x, acc.x), fmaf(x, v.y, acc.y), fmaf(x, v.z, acc.z), fmaf(x, v.w, acc.w));
         }
       }
       __syncthreads();
     }
     if (part == 0 && c < a.head_dim) {
+      const float inv = 1.0f / l;
       const uint2 v = make_uint2(pack2(acc.x * inv, acc.y * inv, T{}), pack2(acc.z * inv, acc.w * inv, T{}));
       *reinterpret_cast<uint2*>(out + c) = some ? v : make_uint2(0u, 0u);
     }
@@ -902,10 +912,10 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
     const JoinArgs j{a.out, a.lens, a.part, s.part, a.ml, s.ml, a.plan, a.batch, a.tokens, a.q_heads, a.kv_heads, a.group,
                      a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, h.rows,
                      h.unit_rows, h.row_tiles, h.tiles, h.run, h.slots, h.unit_rows == h.rows && h.slots > 1};
-    const long long rows = (long long)a.batch * a.tokens * a.q_heads;
-    err = rows < 8LL * device_sm_count()
-              ? launch_pdl(join_rows<T, 8>, dim3((unsigned)rows), dim3(256), 0, stream, j)
-              : launch_pdl(join_rows<T, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, j);
+    const int rows = a.tokens * a.q_heads;
+    err = (long long)rows * a.batch < 8LL * device_sm_count()
+              ? launch_pdl(join_rows<T, 8>, dim3(rows, a.batch), dim3(256), 0, stream, j)
+              : launch_pdl(join_rows<T, 1>, dim3((rows + 7) / 8, a.batch), dim3(256), 0, stream, j);
   }
   if (err != cudaSuccess) {
     cudaGetLastError();
@@ -957,6 +967,7 @@ CKB_EXPORT int ckb_attention_paged_launch(const void* q, const void* key_cache, 
   a.group = q_heads / kv_heads;
   a.head_dim = head_dim;
   a.block_size = block_size;
+  a.block_log = block_size & (block_size - 1) ? -1 : __builtin_ctz(block_size);
   a.table_width = (int)table_width;
   a.prefix = batch == 1 ? 0 : (int)shared_prefix;
   a.rows = z.rows;

@@ -42,11 +42,6 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool elect_one() {
-  unsigned is;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
-  return is != 0u;
-}
 // D (+)= A B, A and B in shared memory.
 __device__ __forceinline__ void tc_mma(unsigned d, uint64_t a, uint64_t b, unsigned kind, bool add) {
   asm volatile(
@@ -197,7 +192,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
       const int pos = tile * kPrefixTile + lane * box_rows;
       if (lane >= pages || pos >= a.prefix) return outside;
-      const int page = pos / a.block_size;
+      const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
       const long long block = __ldg(a.tables + page);
       if (block < 0 || block >= a.num_blocks) return outside;
       return (int)(block * a.block_size + (pos - page * a.block_size));

@@ -34,6 +34,11 @@ __device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap* map, 
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(0), "r"(head)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  unsigned is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0u;
+}
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -138,32 +143,37 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     // Pages of a tile: box_rows rows each, in `blocks` boxes.
     const int box_rows = 1 << rows_log, pages = kTile >> rows_log, blocks = a.head_dim == DT ? 1 : DT / 64;
     const int page_bytes = box_rows * 128 * (DT / 64);
+    const bool leader = elect_one();
     const auto page_of = [&](const Cursor& c) -> int {  // lane p: the cache row where page p of the tile begins
-      const int pos = own_begin(a.prefix, a.tokens, lens[c.b]) + c.tile * kTile + lane * box_rows;
-      if (lane >= pages || pos >= lens[c.b]) return -1;
-      const int page = pos / a.block_size;
+      const int len = lens[c.b], pos = own_begin(a.prefix, a.tokens, len) + c.tile * kTile + lane * box_rows;
+      if (lane >= pages || pos >= len) return -1;
+      const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
       const long long block = __ldg(a.tables + (long long)c.b * a.table_width + page);
       if (block < 0 || block >= a.num_blocks) return (int)(a.num_blocks * a.block_size);  // outside the map: zeros
       return (int)(block * a.block_size + (pos - page * a.block_size));
     };
-    int q_loads = 0;
+    int q_loads = 0, stage = 0, parity = 1;
     int row_now = page_of(at);
     for (int w = first; w < last; ++w) {
-      const int stage = (w - first) % kStages;
-      const int kv_head = at.unit / a.row_tiles;
+      const int kv_head = a.row_tiles == 1 ? at.unit : at.unit / a.row_tiles;
       Cursor ahead = at;
       axis_next(cum, a.batch, units, ahead);
-      const int row_next = w + 1 < last ? page_of(ahead) : -1;  // behind this tile's copies
-      wait_or_give_up(&empty[stage], (((w - first) / kStages) & 1) ^ 1, dead);
+      const int row_next = w + 1 < last ? page_of(ahead) : -1;  // on its way while this tile's copies are issued
+      wait_or_give_up(&empty[stage], parity, dead);
       if (dead) break;
-      const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], there * 2 * page_bytes);
-      for (int i = lane; __any_sync(0xffffffffu, i < pages * blocks * 2); i += 32) {
-        const int page = i % pages, block = i / pages % blocks, is_v = i / (pages * blocks);
+      const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));  // the first pages
+      if (leader) mbar_arrive_expect_tx(&full[stage], there * 2 * page_bytes);
+      const unsigned to = smem_at + stage * 2 * S::kTileBytes;
+#pragma unroll 1
+      for (int page = 0; page < there; ++page) {
         const int row = __shfl_sync(0xffffffffu, row_now, page);
-        if (i < pages * blocks * 2 && row >= 0)
-          tma_load4(smem_at + (stage * 2 + is_v) * S::kTileBytes + page * page_bytes + block * (box_rows * 128),
-                    is_v ? &value_map : &key_map, block * 64, row, kv_head, &full[stage]);
+        if (leader) {
+          for (int block = 0; block < blocks; ++block) {
+            const unsigned dst = to + page * page_bytes + block * (box_rows * 128);
+            tma_load4(dst, &key_map, block * 64, row, kv_head, &full[stage]);
+            tma_load4(dst + S::kTileBytes, &value_map, block * 64, row, kv_head, &full[stage]);
+          }
+        }
       }
       if (w == first || at.tile == 0) {  // a piece begins: its queries come with its first tile
         const int row0 = (at.unit - kv_head * a.row_tiles) * kRows;
@@ -172,15 +182,19 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
           const Row x = row_of<false>(a, at.b, kv_head, row0 + r);
           const bool fill = x.real && chunk * 8 < a.head_dim;
           const long long off = fill ? x.b * a.vq.batch + x.t * a.vq.token + x.head * a.vq.head + chunk * 8 : 0;
-          copy16(smem_at + S::kOffQ + (q_loads % kStages) * S::kQBytes + at_chunk<DT>(r, chunk), (const T*)a.q + off, fill);
+          copy16(smem_at + S::kOffQ + q_loads * S::kQBytes + at_chunk<DT>(r, chunk), (const T*)a.q + off, fill);
         }
-        ++q_loads;
+        q_loads = q_loads + 1 == kStages ? 0 : q_loads + 1;
         mbar_arrive_copies(&full[stage]);
       } else {
         mbar_arrive(&full[stage]);
       }
       at = ahead;
       row_now = row_next;
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
     copy_commit();
     copy_wait<0>();
@@ -197,12 +211,11 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   }
   constexpr int kNt = kKeys / 8, kDt = DT / 8;
   float o[kDt][4], m[2], l[2];
-  int len = 0, begin = 0, min_limit = 0, lim[2] = {0, 0}, q_now = 0, piece_begin = 0;
+  int len = 0, begin = 0, min_limit = 0, lim[2] = {0, 0}, q_now = -1, piece_begin = 0, stage = 0, parity = 0;
   for (int w = first; w < last; ++w) {
-    const int stage = (w - first) % kStages;
-    const int kv_head = at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
+    const int kv_head = a.row_tiles == 1 ? at.unit : at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
     if (w == first || at.tile == 0) {  // a new piece
-      ++q_now;
+      q_now = q_now + 1 == kStages ? 0 : q_now + 1;
       piece_begin = at.tile;
       len = lens[at.b];
       begin = own_begin(a.prefix, a.tokens, len);
@@ -219,10 +232,10 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
     }
-    wait_or_give_up(&full[stage], ((w - first) / kStages) & 1, dead);
+    wait_or_give_up(&full[stage], parity, dead);
 
     const unsigned k_at = smem_at + stage * 2 * S::kTileBytes, v_at = k_at + S::kTileBytes;
-    const unsigned q_at = smem_at + S::kOffQ + ((q_now - 1) % kStages) * S::kQBytes;
+    const unsigned q_at = smem_at + S::kOffQ + q_now * S::kQBytes;
     const int pos0 = begin + at.tile * kTile + wk * kKeys;
     float s[kNt][4];
 #pragma unroll
@@ -403,6 +416,10 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[stage]);
     axis_next(cum, a.batch, units, at);
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
   }
 }
 
