@@ -189,16 +189,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int page_bytes = box_rows * 128 * (DT / 64);
     const int outside = (int)(a.num_blocks * a.block_size);  // rows of zeros, which a weight of zero must meet
     const bool leader = elect_one();
-    const auto page_of = [&](int tile) -> int {  // lane p: the cache row where page p of the tile begins
+    // Lane p looks up page p of a tile a tile ahead, as in attend_stream.
+    long long block_next = -1;
+    int inside_next = 0;
+    const auto look_up = [&](int tile) {
       const int pos = tile * kPrefixTile + lane * box_rows;
-      if (lane >= pages || pos >= a.prefix) return outside;
+      block_next = -1;
+      if (lane >= pages || pos >= a.prefix) return;
       const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
-      const long long block = __ldg(a.tables + page);
-      if (block < 0 || block >= a.num_blocks) return outside;
-      return (int)(block * a.block_size + (pos - page * a.block_size));
+      inside_next = pos - page * a.block_size;
+      block_next = __ldg(a.tables + page);
     };
     int unit = first / p.tiles, tile = first - unit * p.tiles;
-    int row_now = page_of(tile), in_piece = 0, uses0 = 0, uses1 = 0;
+    int in_piece = 0, uses0 = 0, uses1 = 0;
+    look_up(tile);
     for (int w = first; w < last; ++w) {
       // Alternate tiles of a piece have a stage each, that of their group, so that every group meets its stage's phases
       // one after the other.
@@ -209,19 +213,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         tile = in_piece = 0;
         ++unit;
       }
-      const int row_next = page_of(tile);  // on its way while this tile's copies are issued
+      const int row_now =
+          (int)(block_next < 0 || block_next >= a.num_blocks ? outside : block_next * a.block_size + inside_next);
+      look_up(tile);
       wait_or_give_up(&empty[stage], (use & 1) ^ 1, dead);
       if (dead) break;
       if (leader) mbar_arrive_expect_tx(&full[stage], S::kTileBytes);
       const unsigned at = ring + stage * S::kTileBytes;
-#pragma unroll 1
+#pragma unroll 4
       for (int page = 0; page < pages; ++page) {
         const int row = __shfl_sync(0xffffffffu, row_now, page);
         if (leader)
           for (int block = 0; block < blocks; ++block)
             tma_load4(at + page * page_bytes + block * (box_rows * 128), map, block * 64, row, kv_head, &full[stage]);
       }
-      row_now = row_next;
     }
   } else if (warp >= 9) {
     // The whole warp goes through this, so that addresses and descriptors stay in uniform registers; one lane issues.

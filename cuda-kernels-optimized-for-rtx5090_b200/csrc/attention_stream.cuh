@@ -144,27 +144,35 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
     const int box_rows = 1 << rows_log, pages = kTile >> rows_log, blocks = a.head_dim == DT ? 1 : DT / 64;
     const int page_bytes = box_rows * 128 * (DT / 64);
     const bool leader = elect_one();
-    const auto page_of = [&](const Cursor& c) -> int {  // lane p: the cache row where page p of the tile begins
+    // Lane p looks up page p of a tile a tile ahead: the block's id is on its way while the tile before is copied, and only
+    // then becomes the cache row where the page begins.
+    long long block_next = -1;
+    int inside_next = 0;
+    bool there_next = false;
+    const auto look_up = [&](const Cursor& c) {
       const int len = lens[c.b], pos = own_begin(a.prefix, a.tokens, len) + c.tile * kTile + lane * box_rows;
-      if (lane >= pages || pos >= len) return -1;
+      there_next = lane < pages && pos < len;
+      if (!there_next) return;
       const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
-      const long long block = __ldg(a.tables + (long long)c.b * a.table_width + page);
-      if (block < 0 || block >= a.num_blocks) return (int)(a.num_blocks * a.block_size);  // outside the map: zeros
-      return (int)(block * a.block_size + (pos - page * a.block_size));
+      inside_next = pos - page * a.block_size;
+      block_next = __ldg(a.tables + (long long)c.b * a.table_width + page);
     };
     int q_loads = 0, stage = 0, parity = 1;
-    int row_now = page_of(at);
+    look_up(at);
     for (int w = first; w < last; ++w) {
       const int kv_head = a.row_tiles == 1 ? at.unit : at.unit / a.row_tiles;
       Cursor ahead = at;
       axis_next(cum, a.batch, units, ahead);
-      const int row_next = w + 1 < last ? page_of(ahead) : -1;  // on its way while this tile's copies are issued
+      // A block outside the cache lies outside the map: zeros.
+      const int row_now = (int)(block_next < 0 || block_next >= a.num_blocks ? a.num_blocks * a.block_size
+                                                                             : block_next * a.block_size + inside_next);
+      const int there = __popc(__ballot_sync(0xffffffffu, there_next));  // the first pages
+      if (w + 1 < last) look_up(ahead);
       wait_or_give_up(&empty[stage], parity, dead);
       if (dead) break;
-      const int there = __popc(__ballot_sync(0xffffffffu, row_now >= 0));  // the first pages
       if (leader) mbar_arrive_expect_tx(&full[stage], there * 2 * page_bytes);
       const unsigned to = smem_at + stage * 2 * S::kTileBytes;
-#pragma unroll 1
+#pragma unroll 4
       for (int page = 0; page < there; ++page) {
         const int row = __shfl_sync(0xffffffffu, row_now, page);
         if (leader) {
@@ -190,7 +198,6 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
         mbar_arrive(&full[stage]);
       }
       at = ahead;
-      row_now = row_next;
       if (++stage == kStages) {
         stage = 0;
         parity ^= 1;
