@@ -28,10 +28,15 @@ namespace {
 constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
 constexpr int kMaxShared = 232448;  // bytes of shared memory that a CTA can have
-#ifndef CKB_PREFIX_SHARE
-#define CKB_PREFIX_SHARE 6
-#endif
-constexpr int kPrefixShare = CKB_PREFIX_SHARE;  // eighths of the SMs that the shared work takes
+// The shared work takes at most 7 of 8 SMs, so that own tokens are read from its first moment on, and runs of at least 4 tiles,
+// as a CTA spends 5 us before its first tile and 3 us on its piece: 64 sequences behind 4096 tokens take 45 us so, 49 us with
+// runs of 3 and 54 us with runs of 8; 256 behind 16384 138 us with 7 of 8 SMs, 147 us with 6, 172 us with 5.
+constexpr int kPrefixShare = 7;
+constexpr int kPrefixRun = 4;
+// What the shared work's CTAs are expected to take: 9 us and 1.9 us a tile (half where its groups share the tiles). The own
+// work's CTAs that start beside them get so many more tiles, of 1.5 us, than those that come after (without: 51 us instead of
+// 45 us in the first case). These only balance the load.
+constexpr int kPrefixCtaNs = 9000, kPrefixTileNs = 1900, kOwnTileNs = 1500;
 constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -45,7 +50,7 @@ struct Args {
   void* out;
   float* part;     // [slots][rows of a tile][D] of this launch's pieces
   float2* ml;      // [slots][rows of a tile]: (m in powers of 2, l)
-  int* plan;       // own work only: [batch + 1] running tile counts, then the tiles of a run
+  int* plan;       // own work only: [batch + 1] running tile counts, then the runs
   View3 vq;
   long long num_blocks;
   int batch, tokens, q_heads, kv_heads, group, head_dim, block_size, table_width;
@@ -55,6 +60,7 @@ struct Args {
   int row_tiles;   // row tiles of a unit's rows
   float scale_log2;
   bool beside;     // own work launched beside the shared work: see start_all
+  int early, ahead;  // CTAs of the own work that start with the shared work, tiles they are expected to do before the others start
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -199,6 +205,30 @@ __device__ __forceinline__ void own_axis(const Args& a, int units, int* cum, int
   if (tid == 0) cum[a.batch] = before;
   __syncthreads();
 }
+// How the axis of `all` tiles is cut for `ctas` CTAs: the first `early` have runs of `longer` tiles, the others of `run`.
+struct Runs {
+  int early, longer, run;
+  __device__ __forceinline__ int begin(int cta, int all) const {
+    const long long w = cta < early ? (long long)cta * longer : (long long)early * longer + (long long)(cta - early) * run;
+    return (int)min(w, (long long)all);
+  }
+  __device__ __forceinline__ int cta_of(int w) const {
+    return w < early * longer ? w / longer : early + (w - early * longer) / run;
+  }
+};
+__device__ __forceinline__ Runs runs_of(const Args& a, int all, int ctas) {
+  Runs r;
+  r.early = a.early;
+  const int rest = all - (int)min((long long)a.early * a.ahead, (long long)all);
+  if (rest > 0 || a.early == 0) {
+    r.run = max(1, (rest + ctas - 1) / ctas);
+    r.longer = r.run + a.ahead;
+  } else {  // the early ones do it all
+    r.run = 1;
+    r.longer = max(1, (all + a.early - 1) / a.early);
+  }
+  return r;
+}
 // Tile w of the axis of `seqs` sequences (w < cum[seqs]).
 __device__ __forceinline__ Cursor axis_start(const int* cum, int seqs, int units, int w) {
   int lo = 0, hi = seqs;  // the last b with cum[b] <= w
@@ -224,6 +254,17 @@ __device__ __forceinline__ void axis_next(const int* cum, int seqs, int units, C
     ++c.b;
     c.tiles = c.b < seqs ? (cum[c.b + 1] - cum[c.b]) / units : 1;
   } while (c.b < seqs && c.tiles == 0);
+}
+
+// What the join needs to know of the own work's cuts.
+template <int kCount>
+__device__ __forceinline__ void write_plan(const Args& a, const int* cum, const Runs& r) {
+  for (int b = threadIdx.x; b <= a.batch; b += kCount) a.plan[b] = cum[b];
+  if (threadIdx.x == 0) {
+    a.plan[a.batch + 1] = r.early;
+    a.plan[a.batch + 2] = r.longer;
+    a.plan[a.batch + 3] = r.run;
+  }
 }
 
 // Writes a lane's part of row half i of an accumulator o: the output itself where the piece is the whole unit, else the
@@ -298,13 +339,9 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   }
   __syncthreads();
   const int all = cum[seqs];
-  const int run = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
-  if (!kShared && blockIdx.x == 0) {
-    for (int b = tid; b <= a.batch; b += kThreads) a.plan[b] = cum[b];
-    if (tid == 0) a.plan[a.batch + 1] = run;
-  }
-  const int first = (int)min((long long)blockIdx.x * run, (long long)all);
-  const int last = min(first + run, all);
+  const Runs runs = runs_of(a, all, gridDim.x);
+  if (!kShared && blockIdx.x == 0) write_plan<kThreads>(a, cum, runs);
+  const int first = runs.begin(blockIdx.x, all), last = runs.begin(blockIdx.x + 1, all);
   if (!kShared && a.beside && blockIdx.x == 0 && first >= last) pdl_wait();
   if (first >= last) return;
 
@@ -607,15 +644,16 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
 
   // Own pieces: slots own_slot, own_slot + 1, ...; shared ones the same.
   const int units = a.kv_heads * a.own_row_tiles, unit = kv_head * a.own_row_tiles + in / a.own_rows;
-  const int begin = a.plan[b], tiles = (a.plan[b + 1] - begin) / units, run = a.plan[a.batch + 1];
+  const int begin = a.plan[b], tiles = (a.plan[b + 1] - begin) / units;
+  const Runs runs{a.plan[a.batch + 1], a.plan[a.batch + 2], a.plan[a.batch + 3]};
   const long long n = a.lens[b];
   const int len = (int)(n < 0 ? 0 : n < a.table_positions ? n : a.table_positions);
   const bool sharing = a.shared_row_tiles > 0 && own_begin(a.prefix, a.tokens, len) > 0;
   int own = 0;
   long long own_at = 0;  // workspace row of the first own piece
   if (tiles > 0) {
-    const int w0 = begin + unit * tiles, c0 = w0 / run;
-    own = (w0 + tiles - 1) / run - c0 + 1;
+    const int w0 = begin + unit * tiles, c0 = runs.cta_of(w0);
+    own = runs.cta_of(w0 + tiles - 1) - c0 + 1;
     own_at = ((long long)b * units + unit + c0) * a.own_rows + in % a.own_rows;
     if (own == 1 && !sharing) return;  // written out by its CTA (the same for all warps of the row)
   }
@@ -747,13 +785,14 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
     const long long all = (long long)h.tiles * kv_heads * h.row_tiles;
     if (all > INT_MAX / 2) return false;
     h.run = (int)((all + at_once - 1) / at_once);
+    if (i == 0 && h.run < kPrefixRun) h.run = kPrefixRun < h.tiles ? kPrefixRun : h.tiles;
     h.ctas = (int)((all + h.run - 1) / h.run);
     const long long need = ((long long)kv_heads * h.row_tiles + h.ctas) * h.slots * h.rows;
     if (need > shared_rows) shared_rows = need;
   }
   const auto up = [](long long n) { return (n + 255) / 256 * 256; };
   z.off_plan = 0;
-  z.off_own_ml = up((batch + 2) * 4);
+  z.off_own_ml = up((batch + 4) * 4);
   z.off_own = z.off_own_ml + up(z.own_slots * z.own_rows * 8);
   z.off_shared_ml = z.off_own + up(z.own_slots * z.own_rows * head_dim * 4);
   z.off_shared = z.off_shared_ml + up(shared_rows * 8);
@@ -862,8 +901,9 @@ cudaError_t start_own(const Args& a, int warps, int ctas, const Maps& maps, cuda
 }
 
 template <typename T, int DT>
-cudaError_t start_prefix(const Args& a, const Sizes& z, cudaStream_t stream) {
-  const Maps maps = maps_of<T>(a, a.block_size == 8 ? 3 : 4);
+cudaError_t start_prefix(const Args& a, const Sizes& z, const Maps& own_maps, cudaStream_t stream) {
+  const int rows_log = a.block_size == 8 ? 3 : 4;
+  const Maps maps = own_maps.rows_log == rows_log ? own_maps : maps_of<T>(a, rows_log);
   if (!maps.fit) return cudaErrorInvalidValue;
   const auto& h = z.shared[0];
   const int bytes = PrefixShape<DT>::kBytes;
@@ -890,6 +930,10 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
   cudaError_t err = cudaSuccess;
   Args s = a;
   a.beside = a.prefix > 0;
+  if (a.beside && tensor && h.ctas < device_sm_count()) {
+    a.early = (device_sm_count() - h.ctas) * per_sm(a.head_dim);
+    a.ahead = (kPrefixCtaNs + h.run * (h.unit_rows == h.rows ? kPrefixTileNs / 2 : kPrefixTileNs)) / kOwnTileNs;
+  }
   a.row_tiles = z.own_row_tiles;
   a.part = reinterpret_cast<float*>(work + z.off_own);
   a.ml = reinterpret_cast<float2*>(work + z.off_own_ml);
@@ -898,7 +942,7 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
   s.ml = reinterpret_cast<float2*>(work + z.off_shared_ml);
   if (a.prefix > 0) {
     if (tensor)
-      err = dt == 64 ? start_prefix<T, 64>(s, z, stream) : start_prefix<T, 128>(s, z, stream);
+      err = dt == 64 ? start_prefix<T, 64>(s, z, maps, stream) : start_prefix<T, 128>(s, z, maps, stream);
     else
       err = dt == 64 ? start<T, 64, 4, true>(s, h.ctas, stream)
             : dt == 128 ? start<T, 128, 4, true>(s, h.ctas, stream)

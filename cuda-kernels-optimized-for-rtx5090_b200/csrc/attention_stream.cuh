@@ -124,13 +124,9 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1))
   const int units = a.kv_heads * a.row_tiles;
   own_axis<kAll>(a, units, cum, lens, reinterpret_cast<int*>(ml_sh));  // its barriers order the mbarriers' set-up too
   const int all = cum[a.batch];
-  const int run = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= a.batch; b += kAll) a.plan[b] = cum[b];
-    if (tid == 0) a.plan[a.batch + 1] = run;
-  }
-  const int first = (int)min((long long)blockIdx.x * run, (long long)all);
-  const int last = min(first + run, all);
+  const Runs runs = runs_of(a, all, gridDim.x);
+  if (blockIdx.x == 0) write_plan<kAll>(a, cum, runs);
+  const int first = runs.begin(blockIdx.x, all), last = runs.begin(blockIdx.x + 1, all);
   // The first CTA, which always has a loading warp, ends after the shared work.
   if (first >= last) {
     if (a.beside && blockIdx.x == 0) pdl_wait();
