@@ -7,37 +7,38 @@ sequences of the batch share and that is then read once for the whole batch. No 
 library's C entry is ckb_attention_paged_launch.
 """
 
-import ctypes
+import struct
 
 import torch
 
 from . import _native
 
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
-_STRIDES = ctypes.c_longlong * 3
+_STRIDES = struct.Struct("3q")
 
 
 def _problem(q, key_cache, value_cache, tables, lens, prefix):
     """Why these inputs are not an attention these kernels serve, or None."""
-    if q.dtype not in _DTYPES or q.dim() != 4 or min(q.shape[1:]) < 1:
-        return f"q {q.dtype} {tuple(q.shape)}, bf16 or fp16 [B, T, Hq, D] is served"
-    batch, _, q_heads, head_dim = q.shape
+    q_shape, shape, dtype = q.shape, key_cache.shape, q.dtype
+    if dtype not in _DTYPES or len(q_shape) != 4 or min(q_shape[1:]) < 1:
+        return f"q {dtype} {tuple(q_shape)}, bf16 or fp16 [B, T, Hq, D] is served"
+    batch, _, q_heads, head_dim = q_shape
     if head_dim % 8 or head_dim > 256:
         return f"head_dim {head_dim}, a multiple of 8 up to 256 is served"
+    if shape != value_cache.shape:
+        return f"key_cache {tuple(shape)} and value_cache {tuple(value_cache.shape)} differ"
     for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
-        if c.dtype != q.dtype or c.dim() != 4 or c.shape[3] != head_dim or c.shape[1] < 1 or c.shape[2] < 1 or \
+        if c.dtype != dtype or len(shape) != 4 or shape[3] != head_dim or shape[1] < 1 or shape[2] < 1 or \
                 not c.is_contiguous():
-            return (f"{name} must be a contiguous [blocks, block_size, Hkv, {head_dim}] tensor of {q.dtype}, got {c.dtype} "
-                    f"{tuple(c.shape)}")
-    if key_cache.shape != value_cache.shape:
-        return f"key_cache {tuple(key_cache.shape)} and value_cache {tuple(value_cache.shape)} differ"
-    if q_heads % key_cache.shape[2]:
-        return f"{q_heads} query heads for {key_cache.shape[2]} key heads"
+            return (f"{name} must be a contiguous [blocks, block_size, Hkv, {head_dim}] tensor of {dtype}, got {c.dtype} "
+                    f"{tuple(shape)}")
+    if q_heads % shape[2]:
+        return f"{q_heads} query heads for {shape[2]} key heads"
     if tables.dtype != torch.int64 or tables.dim() != 2 or tables.shape[0] != batch or tables.shape[1] < 1:
         return f"block_tables {tables.dtype} {tuple(tables.shape)}, int64 [{batch}, blocks] is needed"
-    if lens.dtype != torch.int64 or tuple(lens.shape) != (batch,):
+    if lens.dtype != torch.int64 or lens.shape != (batch,):
         return f"seq_lens {lens.dtype} {tuple(lens.shape)}, int64 [{batch}] is needed"
-    block_size = key_cache.shape[1]
+    block_size = shape[1]
     if not isinstance(prefix, int) or prefix < 0 or prefix % block_size or prefix > tables.shape[1] * block_size:
         return (f"shared_prefix {prefix!r} must be a number of tokens, a multiple of the block size {block_size}, within the "
                 f"{tables.shape[1]} blocks of a sequence")
@@ -65,7 +66,7 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     if key_cache.data_ptr() % 16 or value_cache.data_ptr() % 16:
         raise ValueError("attention: the caches must start on 16-byte boundaries")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device or \
             out.data_ptr() % 16:
         raise ValueError("attention: out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
@@ -84,9 +85,9 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     if need < 0:
         raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
                          f"block_tables {tuple(tables.shape)}")
-    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    work = q.new_empty((need,), dtype=torch.uint8)
     _native.call(lib.ckb_attention_paged_launch, q, q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-                 tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES(st_b, st_t, st_h),
+                 tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES.pack(st_b, st_t, st_h),
                  batch, tokens, q_heads, kv_heads, head_dim, num_blocks, block_size, width, shared_prefix, scale,
                  _DTYPES[q.dtype])
     return out

@@ -13,9 +13,9 @@ params.json beside this module may set "rows" and "splits" as the reference's do
 and do not change the B200 launch shape.
 """
 
-import ctypes
 import json
 import os
+import struct
 
 import torch
 
@@ -154,7 +154,7 @@ def rope_kv_cache(q, k, v, position_ids, cos, sin, key_cache, value_cache, slot_
     return q_out, k_out
 
 
-_STRIDES = ctypes.c_longlong * 15
+_STRIDES = struct.Struct("15q")  # the 15 strides as the C ABI reads them
 
 
 def _strides(t):
@@ -178,11 +178,15 @@ def _strided(t, name=None):
 def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches, slot_mapping, eps, inplace, write_k, out):
     if (cos is None) != (sin is None) or (cos is None) == (theta is None):
         raise ValueError("rope candidate: give the cos/sin cache (both) or theta")
-    problem = _problem(q, k, cos, sin, position_ids)
-    if problem:
-        raise ValueError(f"rope candidate: {problem}")
-    batch, seq, q_heads, head_dim = q.shape
-    k_shape = k.shape
+    q_shape, k_shape, ids_shape, dtype = q.shape, k.shape, position_ids.shape, q.dtype
+    # What _problem() checks, in the order that a good call passes fastest; it then words what is wrong.
+    if not (len(q_shape) == 4 and len(k_shape) == 4 and dtype in _QK and k.dtype == dtype and
+            position_ids.dtype == torch.int64 and q_shape[:2] == ids_shape and k_shape[:2] == ids_shape and
+            q_shape[3] == k_shape[3] and q_shape[3] % 2 == 0 and
+            (cos is None or (cos.dtype in _CACHE and cos.dtype == sin.dtype and cos.dim() == 2 and cos.shape == sin.shape and
+                             cos.shape[1] == q_shape[3]))):
+        raise ValueError(f"rope candidate: {_problem(q, k, cos, sin, position_ids)}")
+    batch, seq, q_heads, head_dim = q_shape
     kv_heads = k_shape[2]
     if q_heads < 1 or kv_heads < 1 or head_dim < 2:
         raise ValueError(f"rope candidate: shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
@@ -202,15 +206,16 @@ def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches,
     if caches is not None:
         if v.shape != k_shape or v.dtype != k.dtype:
             raise ValueError(f"rope candidate: v {v.dtype} {tuple(v.shape)} must match k {k.dtype} {tuple(k.shape)}")
-        for name, c in zip(("key_cache", "value_cache"), caches):
-            if c.dtype != q.dtype or c.dim() != 4 or c.shape[2:] != k_shape[2:] or not c.is_contiguous():
+        key_cache, value_cache = caches
+        shape = key_cache.shape
+        if shape != value_cache.shape:
+            raise ValueError(f"rope candidate: key_cache {tuple(shape)} and value_cache {tuple(value_cache.shape)} differ")
+        for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
+            if c.dtype != dtype or len(shape) != 4 or shape[2] != kv_heads or shape[3] != head_dim or not c.is_contiguous():
                 raise ValueError(f"rope candidate: {name} must be a contiguous [blocks, block_size, {kv_heads}, "
-                                 f"{head_dim}] tensor of {q.dtype}, got {c.dtype} {tuple(c.shape)}")
-        if caches[0].shape != caches[1].shape:
-            raise ValueError(f"rope candidate: key_cache {tuple(caches[0].shape)} and value_cache "
-                             f"{tuple(caches[1].shape)} differ")
-        if slot_mapping.dtype != torch.int64 or slot_mapping.shape != position_ids.shape:
-            raise ValueError(f"rope candidate: slot_mapping must be int64 {tuple(position_ids.shape)}")
+                                 f"{head_dim}] tensor of {dtype}, got {c.dtype} {tuple(shape)}")
+        if slot_mapping.dtype != torch.int64 or slot_mapping.shape != ids_shape:
+            raise ValueError(f"rope candidate: slot_mapping must be int64 {tuple(ids_shape)}")
         tensors += v, slot_mapping, *caches
     _native.require_cuda("rope", *tensors)
     if inplace:
@@ -219,8 +224,8 @@ def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches,
     else:
         q, k = _strided(q), _strided(k)
         if out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            k_out = torch.empty(k_shape, dtype=q.dtype, device=q.device) if write_k else None
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if write_k else None
         else:
             q_out, k_out = out
             for o, t in ((q_out, q), (k_out, k)):
@@ -236,14 +241,14 @@ def _qk_norm(q, k, v, position_ids, q_weight, k_weight, cos, sin, theta, caches,
     none = (0, 0, 0)
     if caches is not None:
         v, slots = _strided(v), slot_mapping.contiguous()
-        v_at, slots_at, key_at, value_at = v.data_ptr(), slots.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr()
-        cache_slots = caches[0].shape[0] * caches[0].shape[1]
-    strides = _STRIDES(*_strides(q), *_strides(k), *(none if caches is None else _strides(v)), *_strides(q_out),
-                       *(none if k_out is None else _strides(k_out)))
+        v_at, slots_at, key_at, value_at = v.data_ptr(), slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr()
+        cache_slots = shape[0] * shape[1]
+    strides = _STRIDES.pack(*_strides(q), *_strides(k), *(none if caches is None else _strides(v)), *_strides(q_out),
+                            *(none if k_out is None else _strides(k_out)))
     _native.call(_native.load("rope").ckb_rope_qk_norm_launch, q, q.data_ptr(), k.data_ptr(), v_at, q_weight.data_ptr(),
                  k_weight.data_ptr(), cos_at, sin_at, freqs_at, ids.data_ptr(), slots_at, q_out.data_ptr(),
                  None if k_out is None else k_out.data_ptr(), key_at, value_at, strides, positions, cache_slots, batch,
-                 seq, q_heads, kv_heads, head_dim, _QK[q.dtype], w_dtype, cache_dtype, eps)
+                 seq, q_heads, kv_heads, head_dim, _QK[dtype], w_dtype, cache_dtype, eps)
     return q_out, k_out
 
 

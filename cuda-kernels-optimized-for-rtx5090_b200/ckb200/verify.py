@@ -16,18 +16,19 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 def _problem(target, tokens, uniforms, draft, counts):
     """Why these inputs are not a verification these kernels serve, or None."""
-    if target.dtype not in _DTYPES or target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
-        return f"target_probs {target.dtype} {tuple(target.shape)}, fp32 or bf16 [B, K + 1, V] is served"
-    batch, rows, vocab = target.shape
+    shape, dtype = target.shape, target.dtype
+    if dtype not in _DTYPES or len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        return f"target_probs {dtype} {tuple(shape)}, fp32 or bf16 [B, K + 1, V] is served"
+    batch, rows, vocab = shape
     if vocab > 1 << 30 or rows > 1 << 20:
-        return f"target_probs {tuple(target.shape)}"
-    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (batch, rows - 1):
-        return f"draft_tokens {tokens.dtype} {tuple(tokens.shape)} for target_probs {tuple(target.shape)}"
-    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (batch, rows):
+        return f"target_probs {tuple(shape)}"
+    if tokens.dtype != torch.int64 or tokens.shape != (batch, rows - 1):
+        return f"draft_tokens {tokens.dtype} {tuple(tokens.shape)} for target_probs {tuple(shape)}"
+    if uniforms.dtype != torch.float32 or uniforms.shape != (batch, rows):
         return f"uniforms {uniforms.dtype} {tuple(uniforms.shape)}, float32 {(batch, rows)} is needed"
-    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (batch, rows - 1, vocab)):
-        return f"draft_probs {draft.dtype} {tuple(draft.shape)} for target_probs {target.dtype} {tuple(target.shape)}"
-    if counts is not None and (counts.dtype != torch.int64 or tuple(counts.shape) != (batch,)):
+    if draft is not None and (draft.dtype != dtype or draft.shape != (batch, rows - 1, vocab)):
+        return f"draft_probs {draft.dtype} {tuple(draft.shape)} for target_probs {dtype} {tuple(shape)}"
+    if counts is not None and (counts.dtype != torch.int64 or counts.shape != (batch,)):
         return f"num_drafts {counts.dtype} {tuple(counts.shape)}, int64 {(batch,)} is needed"
     return None
 
@@ -58,8 +59,7 @@ def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, num_dr
     _native.require_cuda("verify", target_probs, draft_tokens, uniforms, *given)
     batch, rows, vocab = target_probs.shape
     if out is None:
-        tokens = torch.empty((batch, rows), dtype=torch.int64, device=target_probs.device)
-        accepted = torch.empty((batch,), dtype=torch.int64, device=target_probs.device)
+        tokens, accepted = draft_tokens.new_empty((batch, rows)), draft_tokens.new_empty((batch,))
     else:
         tokens, accepted = out
         for t, shape in ((tokens, (batch, rows)), (accepted, (batch,))):
