@@ -81,7 +81,8 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     num_blocks, block_size, kv_heads, _ = key_cache.shape
     width = tables.shape[1]
     lib = _native.load("attention")
-    need = lib.ckb_attention_workspace(batch, tokens, q_heads, kv_heads, head_dim, block_size, width, shared_prefix)
+    need = _native.on_device(lib.ckb_attention_workspace, q, batch, tokens, q_heads, kv_heads, head_dim, block_size, width,
+                             shared_prefix)
     if need < 0:
         raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
                          f"block_tables {tuple(tables.shape)}")

@@ -111,6 +111,7 @@ SHARED = [  # dtype, T, Hq, Hkv, D, block size, prefix, lengths in all
     (HF, 1, 16, 2, 64, 8, 1000, [1001 + i for i in range(40)]),
     (BF, 1, 8, 2, 96, 16, 272, [280, 300]),
     (BF, 1, 160, 160, 64, 16, 144, [145, 160]),  # more units than CTAs
+    (BF, 300, 8, 2, 64, 16, 128, [500, 428]),  # many tokens each
 ]
 
 
@@ -190,9 +191,10 @@ def test_bad_blocks_read_as_zeros_and_lengths_are_clamped():
     assert none.shape == (0, 2, 4, 64)
 
 
-def test_offsets_beyond_32_bits():
+@pytest.mark.parametrize("bs", [16, 24])  # a whole page as a box, and copies of 16 bytes
+def test_offsets_beyond_32_bits(bs):
     """A cache of 2^31 + elements; the sequence's blocks are its last ones. The shared prefix's too."""
-    hkv, d, bs = 8, 128, 16
+    hkv, d = 8, 128
     blocks = (1 << 31) // (hkv * d * bs) + 40
     caches = [torch.empty(blocks, bs, hkv, d, dtype=BF, device="cuda") for _ in range(2)]
     g = torch.Generator().manual_seed(9)
@@ -201,9 +203,37 @@ def test_offsets_beyond_32_bits():
         c[-20:] = s.cuda()
     tables = torch.stack([torch.arange(10), torch.cat([torch.arange(4), torch.arange(10, 16)])])
     q, lens = torch.randn(2, 1, 16, d, generator=g).to(BF), torch.tensor([150, 145])
-    for prefix in (0, 64):
+    for prefix in (0, 4 * bs):
         got = attention.paged_attention(q.cuda(), *caches, (tables + blocks - 20).cuda(), lens.cuda(), shared_prefix=prefix)
         assert_near(got, q, *small, tables, lens, prefix)
+
+
+@pytest.mark.parametrize("bs", [16, 24])
+@pytest.mark.parametrize("t,hq,hkv,d", [(1, 2, 2, 64), (17, 2, 1, 256), (9, 2, 1, 256), (1, 4, 1, 128)])
+def test_the_largest_batch(t, hq, hkv, d, bs):
+    """4096 sequences of up to 40 tokens: the lengths and tile counts of all lie in shared memory, whose limit the wide heads
+    with many rows come nearest to."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    b, n = 4096, 48
+    width = n // bs
+    tables = torch.randperm(b * width, generator=g, device="cuda").view(b, width)
+    caches = [torch.randn(b * width, bs, hkv, d, generator=g, device="cuda").to(BF) for _ in range(2)]
+    lens = torch.randint(0, 41, (b,), generator=g, device="cuda")
+    q = torch.randn(b, t, hq, d, generator=g, device="cuda").to(BF)
+    got = attention.paged_attention(q, *caches, tables, lens)
+    k, v = (c[tables].view(b, n, hkv, d).permute(0, 2, 1, 3).double() for c in caches)
+    x = q.double().view(b, t, hkv, hq // hkv, d).permute(0, 2, 1, 3, 4).reshape(b, hkv, -1, d) @ k.transpose(2, 3) * d ** -0.5
+    limit = (lens[:, None] - t + torch.arange(1, t + 1, device="cuda")).repeat_interleave(hq // hkv, 1)
+    seen = torch.arange(n, device="cuda") < limit[:, None, :, None]
+    p = torch.softmax(x.masked_fill(~seen, float("-inf")), -1).nan_to_num()
+
+    def back(y):
+        return y.view(b, hkv, t, hq // hkv, d).permute(0, 2, 1, 3, 4).reshape(b, t, hq, d)
+
+    want, size = back(p @ v), back(p @ v.abs())
+    a = d ** -0.5 * q.double().abs().sum(-1).max() * k.abs().max()
+    bound = 2.0 ** -8 * (want.abs() + size) + 2 * size * ((d / 16 + 20) * 2.0 ** -23 * a + 2.0 ** -18)
+    assert ((got.double() - want).abs() <= bound + 1e-30).all()
 
 
 def test_streams_repeats_and_graphs_that_share_a_pool():
