@@ -7,15 +7,18 @@
 // x, m, l and o are fp32; the weights exp(x - m) are rounded to the cache's dtype for the product with v (half a step of
 // that dtype on each, as the output's own rounding), q, k and v enter the products as they are.
 //
-// Two kinds of work, of tiles of kTile positions:
-//   own     the positions behind the prefix: a unit is (sequence, kv head, up to 64 of its T * group rows), its positions
-//           are the sequence's own. Bound by the bytes of the cache: every key and value is read once, by one CTA;
+// Two kinds of work:
+//   own     the positions behind the prefix: a unit is (sequence, kv head, up to 64 of its T * group rows), its tiles are 64
+//           of the sequence's own positions. Bound by the bytes of the cache: every key and value is read once, by one CTA
+//           (attend_stream; attend_tiles for block sizes that a TMA box does not fit, about 0.65 of its rate);
 //   shared  the prefix's positions: a unit is (kv head, rows of ALL sequences), so each key and value of the prefix is
-//           read once for many rows, not once for every sequence.
-// The tiles of all units are laid end to end and cut into equal runs, one for each CTA (the own lengths are only known on
-// the device: every CTA adds them up itself). So unequal lengths and few sequences fill the GPU alike. A run's part of a
-// unit is a piece; pieces go to the workspace at slot (unit + CTA), which is different for each, and join_rows joins
-// them. A whole unit, where no prefix is shared, is written out at once.
+//           read once for many rows, not once for every sequence (attend_prefix on tcgen05; attend_tiles for heads of
+//           more than 128 columns and those block sizes). Sequences that end before the prefix does take no part: all their
+//           positions are own ones.
+// The tiles of all units are laid end to end and cut into runs, one for each CTA (the own lengths are only known on the
+// device: every CTA adds them up itself). So unequal lengths and few sequences fill the GPU alike. A run's part of a unit is
+// a piece; pieces go to the workspace at slot (unit + CTA), which is different for each, and join_rows joins them. A whole
+// unit of a sequence that shares no prefix is written out at once.
 #include "ckb200_attention.h"
 #include "common.cuh"
 

@@ -1,4 +1,5 @@
-// Shared device and host helpers for the four row-wise kernels (softmax, RMSNorm, RoPE, top-k) built for sm_100a.
+// Shared device and host helpers for the kernels (softmax, RMSNorm, RoPE, top-k, attention, draft verification) built for
+// sm_100a.
 //
 // Conventions every library in this directory follows (the reference's C ABI, e.g. rmsnorm/kernel.cu:132-139):
 //   * dtype codes: 0 = fp32, 1 = bf16, 2 = fp16;
