@@ -31,6 +31,7 @@ namespace {
 constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
 constexpr int kMaxShared = 232448;  // bytes of shared memory that a CTA can have
+constexpr int kSmShared = 233472;   // and an SM has
 // The shared work takes at most 7 of 8 SMs, so that own tokens are read from its first moment on, and runs of at least 4 tiles,
 // as a CTA spends 5 us before its first tile and 3 us on its piece: 64 sequences behind 4096 tokens take 45 us so, 49 us with
 // runs of 3 and 54 us with runs of 8; 256 behind 16384 138 us with 7 of 8 SMs, 147 us with 6, 172 us with 5.
@@ -63,7 +64,8 @@ struct Args {
   int row_tiles;   // row tiles of a unit's rows
   float scale_log2;
   bool beside;     // own work launched beside the shared work: see start_all
-  int early, ahead;  // CTAs of the own work that start with the shared work, tiles they are expected to do before the others start
+  // CTAs of the own work that start with the shared work, tiles that they are expected to do before the others start.
+  int early, ahead;
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -342,7 +344,8 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   }
   __syncthreads();
   const int all = cum[seqs];
-  const Runs runs = runs_of(a, all, gridDim.x);
+  // The join knows the shared work's runs from the host, which cuts them the same way.
+  const Runs runs = kShared ? Runs{0, 1, (all + (int)gridDim.x - 1) / (int)gridDim.x} : runs_of(a, all, gridDim.x);
   if (!kShared && blockIdx.x == 0) write_plan<kThreads>(a, cum, runs);
   const int first = runs.begin(blockIdx.x, all), last = runs.begin(blockIdx.x + 1, all);
   if (!kShared && a.beside && blockIdx.x == 0 && first >= last) pdl_wait();
@@ -747,14 +750,22 @@ __global__ void __launch_bounds__(256) join_rows(const JoinArgs a) {
 // Host side.
 // ---------------------------------------------------------------------------------------------------------------
 struct Sizes {
-  int rows, own_warps, own_rows, own_row_tiles, own_ctas;
+  int rows, own_warps, own_rows, own_row_tiles, own_per_sm, own_ctas;
   // The shared work on the tensor cores of the fifth generation (0), or by attend_tiles (1).
   struct { int unit_rows, row_tiles, tiles, ctas, run, rows, slots; } shared[2];
   long long own_slots, off_plan, off_own_ml, off_own, off_shared_ml, off_shared, bytes;
 };
 
-// CTAs of attend_tiles on an SM, by shared memory: 2 or 3 stages of 16, 32 or 64 KB for head_dim up to 64, 128 and 256.
-int per_sm(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1; }
+// CTAs of the own work that an SM holds (attend_tiles' own are near enough).
+template <int DT>
+int per_sm_of(int warps, int batch) {
+  return warps == 1 ? Ring<DT, 1>::per_sm(batch) : warps == 2 ? Ring<DT, 2>::per_sm(batch) : Ring<DT, 4>::per_sm(batch);
+}
+int per_sm(int head_dim, int warps, int batch) {
+  return head_dim <= 64    ? per_sm_of<64>(warps, batch)
+         : head_dim <= 128 ? per_sm_of<128>(warps, batch)
+                           : per_sm_of<256>(warps, batch);
+}
 
 bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_dim, int block_size, long long table_width,
               long long prefix, Sizes& z) {
@@ -773,7 +784,8 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
   z.own_row_tiles = (int)((rows + z.own_rows - 1) / z.own_rows);
   const long long tiles = (table_width * block_size + kTile - 1) / kTile;
   if (tiles * batch * kv_heads * z.own_row_tiles > INT_MAX / 2) return false;
-  const int most = device_sm_count() * per_sm(head_dim);
+  z.own_per_sm = per_sm(head_dim, z.own_warps, (int)batch);
+  const int most = device_sm_count() * z.own_per_sm;
   z.own_ctas = most;
   z.own_slots = batch * kv_heads * z.own_row_tiles + z.own_ctas;
   long long shared_rows = 0;  // of the workspace
@@ -934,7 +946,7 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
   Args s = a;
   a.beside = a.prefix > 0;
   if (a.beside && tensor && h.ctas < device_sm_count()) {
-    a.early = (device_sm_count() - h.ctas) * per_sm(a.head_dim);
+    a.early = (device_sm_count() - h.ctas) * z.own_per_sm;
     a.ahead = (kPrefixCtaNs + h.run * (h.unit_rows == h.rows ? kPrefixTileNs / 2 : kPrefixTileNs)) / kOwnTileNs;
   }
   a.row_tiles = z.own_row_tiles;

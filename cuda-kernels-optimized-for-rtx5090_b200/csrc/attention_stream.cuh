@@ -4,7 +4,7 @@
 // attend_tiles from their rate was instructions: 128 threads spent two thirds of them on addresses and copies of 16 bytes,
 // and a block barrier per tile held the warps in step (48 sequences of up to 16001 tokens: 389 us, 4.1 TB/s). Here one
 // warp looks the pages up and issues a TMA box for each page and 64 columns, and the four others only multiply; each
-// goes on as soon as a tile has arrived (mbarriers), whatever the others do: 258 us, 6.1 TB/s or 0.95 of the measured copy
+// goes on as soon as a tile has arrived (mbarriers), whatever the others do: 252 us, 6.3 TB/s or 0.97 of the measured copy
 // bandwidth. With short sequences the 2.5 us before a CTA's first tile, the 0.7 us at the end of each piece and half-filled
 // last tiles show (256 sequences of 256 tokens on average: 4.3 TB/s).
 //
@@ -87,26 +87,35 @@ struct Ring {
   static constexpr int kRows = 16 * WR;
   static constexpr int kKeyWarps = 4 / WR;
   static constexpr int kKeys = kTile / kKeyWarps;
-  static constexpr int kStages = WR == 1 && DT <= 128 ? 3 : 2;
+  static constexpr int kStages = WR == 1 && DT <= 64 ? 3 : 2;
   static constexpr int kTileBytes = kTile * DT * 2;
   static constexpr int kQBytes = kRows * DT * 2;
   static constexpr int kOffQ = kStages * 2 * kTileBytes;
   static constexpr int kOffMl = kOffQ + kStages * kQBytes;
   static constexpr int kOffBars = kOffMl + kKeyWarps * kRows * 8;
   static constexpr int kOffCum = kOffBars + 2 * kStages * 8;
-  static int bytes(int batch) { return kOffCum + (2 * batch + 1) * 4 + 1024; }  // 1024: the tiles' alignment
+  static constexpr int bytes(int batch) { return kOffCum + (2 * batch + 1) * 4; }
+  // CTAs of an SM by registers (with two stages of 32 KB each three CTAs keep as many bytes in flight as two with three
+  // stages, and 12 warps multiply instead of 8: 64 sequences behind 4096 tokens 45.6 -> 42.0 us, 48 ragged ones 259 -> 252;
+  // one of 8192 tokens, whose CTAs have an SM for themselves, 11.9 -> 13.1).
+  static constexpr int kPerSm = DT <= 64 ? 4 : DT <= 128 ? (WR == 1 ? 3 : 2) : 1;
+  // ... and by shared memory, of which the system takes 1 KB for each.
+  static int per_sm(int batch) {
+    const int fit = kSmShared / (bytes(batch) + 1024);
+    return fit < 1 ? 1 : fit < kPerSm ? fit : kPerSm;
+  }
 };
 
-// Heads of up to 64 columns run four CTAs an SM (96 registers; the compiler's own 127 left room for three, and the fourth
-// came after them: 18 x 5 tokens behind 1536 took 21.9 us instead of 17.8 us).
+// The bound matters: at the compiler's own 127 registers for heads of 64 columns three CTAs fitted an SM and the fourth came
+// after them (18 x 5 tokens behind 1536 took 21.9 us instead of 17.8 us).
 template <typename T, int DT, int WR>
-__global__ void __launch_bounds__(32 * (kConsumers + 1), DT <= 64 ? 4 : DT <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     attend_stream(const Args a, int rows_log, const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map) {
   using S = Ring<DT, WR>;
   constexpr int kRows = S::kRows, kKeys = S::kKeys, kStages = S::kStages;
   constexpr int kAll = 32 * (kConsumers + 1);
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) unsigned char tiles[];  // 1024: the swizzle's period
+  unsigned char* smem = tiles;
   float2* ml_sh = reinterpret_cast<float2*>(smem + S::kOffMl);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
   uint64_t* empty = full + kStages;
