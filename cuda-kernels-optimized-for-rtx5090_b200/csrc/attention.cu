@@ -32,15 +32,16 @@ constexpr int kTile = 64;      // positions of a tile
 constexpr int kThreads = 128;  // four warps
 constexpr int kMaxShared = 232448;  // bytes of shared memory that a CTA can have
 constexpr int kSmShared = 233472;   // and an SM has
-// The shared work takes at most 7 of 8 SMs, so that own tokens are read from its first moment on, and runs of at least 4 tiles,
-// as a CTA spends 5 us before its first tile and 3 us on its piece: 64 sequences behind 4096 tokens take 45 us so, 49 us with
-// runs of 3 and 54 us with runs of 8; 256 behind 16384 138 us with 7 of 8 SMs, 147 us with 6, 172 us with 5.
+// The shared work takes at most 7 of 8 SMs, so that own tokens are read from its first moment on (256 sequences behind 16384
+// tokens 128 us, with 6 of 8 SMs 131 us, with all 135 us), and runs of at least 4 tiles, as a CTA spends 5 us before its
+// first tile and 3 us on its piece (64 sequences behind 4096 tokens with up to 1023, up to 32 own tokens: 42 and 21 us; runs of 3
+// tiles 45 and 25 us, of 8 tiles 41 and 27 us).
 constexpr int kPrefixShare = 7;
 constexpr int kPrefixRun = 4;
 // What the shared work's CTAs are expected to take: 9 us and 1.9 us a tile (half where its groups share the tiles). The own
-// work's CTAs that start beside them get so many more tiles, of 1.5 us, than those that come after (without: 51 us instead of
-// 45 us in the first case). These only balance the load.
-constexpr int kPrefixCtaNs = 9000, kPrefixTileNs = 1900, kOwnTileNs = 1500;
+// work's CTAs that start beside them get so many more tiles, of 2 us, than those that come after (64 behind 4096: 42 us, without
+// 50 us; tiles of 1.5 or 2.6 us 44 us). These only balance the load.
+constexpr int kPrefixCtaNs = 9000, kPrefixTileNs = 1900, kOwnTileNs = 2000;
 constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
