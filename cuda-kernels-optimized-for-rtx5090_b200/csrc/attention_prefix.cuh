@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       w += count;
     }
   }
+  settle(dead);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -53,6 +53,12 @@ __device__ __forceinline__ void wait_or_give_up(uint64_t* bar, unsigned parity, 
     atomicOr(&g_attention_status, CKB_STATUS_TIMEOUT);
   }
 }
+// Before a CTA that gave up ends: 10 ms for the copies and products that it may have in flight.
+__device__ __forceinline__ void settle(bool dead) {
+  if (!dead) return;
+#pragma unroll 1
+  for (int i = 0; i < 100; ++i) __nanosleep(100000);
+}
 __device__ __forceinline__ void sync_warps(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // A tile in shared memory: boxes of R = 2^rows_log rows, each DT / 64 blocks of [R][128 bytes], 16-byte chunks exchanged
@@ -214,6 +220,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     }
     copy_commit();
     copy_wait<0>();
+    settle(dead);
     if (a.beside && blockIdx.x == 0) pdl_wait();
     return;
   }
@@ -437,6 +444,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
       parity ^= 1;
     }
   }
+  settle(dead);
 }
 
 }  // namespace

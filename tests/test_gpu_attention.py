@@ -270,6 +270,38 @@ def test_streams_repeats_and_graphs_that_share_a_pool():
     assert bits_equal(outs[0], attention.paged_attention(*a, shared_prefix=64))
 
 
+def test_calls_one_upon_another():
+    """Calls of different sizes back to back on one stream (which recycle each other's workspace while the one before still
+    joins), with the queries and the cache rewritten by other kernels in between, and on two streams at once: every
+    output has the bits of a call alone."""
+    sizes = [(20, BF, 1, 8, 2, 128, 16, [300 + 37 * i for i in range(24)], 256), (21, HF, 3, 8, 4, 64, 16, [90, 164, 1200], 64),
+             (22, BF, 1, 4, 4, 128, 16, [513] * 40, 512), (23, BF, 2, 16, 2, 128, 16, [5, 40, 900, 77], 0)]
+    cases = [([t.cuda() for t in problem(*c)], c[8]) for c in sizes]
+    wants = []
+    for x, prefix in cases:
+        wants.append(attention.paged_attention(*x, shared_prefix=prefix))
+        torch.cuda.synchronize()
+    got = []
+    for _ in range(12):
+        for x, prefix in cases:
+            q, kc = x[0].clone(), x[1].clone()  # written just before, freed just after
+            got.append(attention.paged_attention(q, kc, *x[2:], shared_prefix=prefix))
+            kc.fill_(float("nan"))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    beside = []
+    for _ in range(12):
+        for x, prefix in cases:
+            got.append(attention.paged_attention(*x, shared_prefix=prefix))
+            with torch.cuda.stream(side):
+                beside.append(attention.paged_attention(*x, shared_prefix=prefix))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert bits_equal(out, wants[i % 4]), i
+    for i, out in enumerate(beside):
+        assert bits_equal(out, wants[i % 4]), i
+
+
 def test_no_wait_has_given_up():
     from ckb200 import _native
 
