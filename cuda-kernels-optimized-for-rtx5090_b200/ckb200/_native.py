@@ -116,6 +116,12 @@ def check(err):
 
 
 def require_cuda(op, *tensors):
+    index = tensors[0].get_device()  # -1 on the CPU
+    for t in tensors:
+        if index < 0 or t.get_device() != index:
+            break
+    else:
+        return
     dev = tensors[0].device
     for t in tensors:
         if not t.is_cuda:

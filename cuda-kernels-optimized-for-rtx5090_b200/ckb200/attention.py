@@ -15,12 +15,13 @@ from . import _native
 
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 _STRIDES = struct.Struct("3q")
+_needs = {}  # (device, sizes) -> bytes of workspace
 
 
 def _problem(q, key_cache, value_cache, tables, lens, prefix):
     """Why these inputs are not an attention these kernels serve, or None."""
     q_shape, shape, dtype = q.shape, key_cache.shape, q.dtype
-    if dtype not in _DTYPES or len(q_shape) != 4 or min(q_shape[1:]) < 1:
+    if dtype not in _DTYPES or len(q_shape) != 4 or q_shape[1] < 1 or q_shape[2] < 1 or q_shape[3] < 1:
         return f"q {dtype} {tuple(q_shape)}, bf16 or fp16 [B, T, Hq, D] is served"
     batch, _, q_heads, head_dim = q_shape
     if head_dim % 8 or head_dim > 256:
@@ -81,11 +82,17 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     num_blocks, block_size, kv_heads, _ = key_cache.shape
     width = tables.shape[1]
     lib = _native.load("attention")
-    need = _native.on_device(lib.ckb_attention_workspace, q, batch, tokens, q_heads, kv_heads, head_dim, block_size, width,
-                             shared_prefix)
-    if need < 0:
-        raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
-                         f"block_tables {tuple(tables.shape)}")
+    sizes = (batch, tokens, q_heads, kv_heads, head_dim, block_size, width, shared_prefix)
+    key = (q.get_device(), sizes)
+    need = _needs.get(key)
+    if need is None:
+        need = _native.on_device(lib.ckb_attention_workspace, q, *sizes)
+        if need < 0:
+            raise ValueError(f"attention: sizes beyond what is served: q {tuple(q.shape)}, caches {tuple(key_cache.shape)}, "
+                             f"block_tables {tuple(tables.shape)}")
+        if len(_needs) > 256:
+            _needs.clear()
+        _needs[key] = need
     work = q.new_empty((need,), dtype=torch.uint8)
     _native.call(lib.ckb_attention_paged_launch, q, q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
                  tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.data_ptr(), need, _STRIDES.pack(st_b, st_t, st_h),
