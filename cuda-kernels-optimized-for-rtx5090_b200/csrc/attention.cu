@@ -757,7 +757,7 @@ struct Sizes {
   long long own_slots, off_plan, off_own_ml, off_own, off_shared_ml, off_shared, bytes;
 };
 
-// CTAs of the own work that an SM holds (attend_tiles' own are near enough).
+// CTAs of the own work that an SM holds (attend_stream).
 template <int DT>
 int per_sm_of(int warps, int batch) {
   return warps == 1 ? Ring<DT, 1>::per_sm(batch) : warps == 2 ? Ring<DT, 2>::per_sm(batch) : Ring<DT, 4>::per_sm(batch);
@@ -964,10 +964,15 @@ int start_all(Args a, const Sizes& z, unsigned char* work, cudaStream_t stream) 
             : dt == 128 ? start<T, 128, 4, true>(s, h.ctas, stream)
                         : start<T, 256, 4, true>(s, h.ctas, stream);
   }
+  int ctas = z.own_ctas;
+  if (!maps.fit) {  // what attend_tiles' larger stages leave room for
+    const int fit = device_sm_count() * (dt == 64 ? 4 : dt == 128 ? 2 : 1);
+    ctas = fit < ctas ? fit : ctas;
+  }
   if (err == cudaSuccess)
-    err = dt == 64 ? start_own<T, 64>(a, z.own_warps, z.own_ctas, maps, stream)
-          : dt == 128 ? start_own<T, 128>(a, z.own_warps, z.own_ctas, maps, stream)
-                      : start_own<T, 256>(a, z.own_warps, z.own_ctas, maps, stream);
+    err = dt == 64 ? start_own<T, 64>(a, z.own_warps, ctas, maps, stream)
+          : dt == 128 ? start_own<T, 128>(a, z.own_warps, ctas, maps, stream)
+                      : start_own<T, 256>(a, z.own_warps, ctas, maps, stream);
   if (err == cudaSuccess) {
     const JoinArgs j{a.out, a.lens, a.part, s.part, a.ml, s.ml, a.plan, a.batch, a.tokens, a.q_heads, a.kv_heads, a.group,
                      a.head_dim, a.prefix, a.rows, a.table_width * a.block_size, z.own_rows, z.own_row_tiles, h.rows,
