@@ -60,8 +60,13 @@ __device__ __forceinline__ void store_remote(double* p, unsigned rank, double v)
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory");
 }
 
-// What one element weighs. A NaN or negative probability weighs nothing, as every comparison with it is false.
-__device__ __forceinline__ double weight(float p, float q) { return p > q ? (double)p - (double)q : 0.0; }
+// A probability that is NaN or negative counts as 0 (fmaxf drops a NaN), the target's and the draft's alike.
+__device__ __forceinline__ float clean(float p) { return fmaxf(p, 0.0f); }
+// What one element weighs: max(p - q, 0) of the cleaned p and q. A p that is NaN, negative or not above q is taken as q.
+__device__ __forceinline__ double weight(float p, float q) {
+  const float less = clean(q);
+  return (double)fmaxf(p, less) - (double)less;
+}
 
 // A lane's columns of one step, as they were loaded (widened only where they are used, so that several steps' loads fit
 // the registers). kVec: one 16-byte vector, else one element. Columns from `end` on are zeros and weigh nothing.
@@ -98,7 +103,12 @@ struct Weights {
     pp.widen(fp);
     pq.widen(fq);
 #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = i + e == without ? 0.0 : weight(fp[e], fq[e]);
+    for (int e = 0; e < N; ++e) w[e] = weight(fp[e], fq[e]);
+    if ((unsigned)(without - i) < (unsigned)N) {  // asked once for all N columns
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i + e == without) w[e] = 0.0;
+    }
   }
 };
 
@@ -176,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_rows(const VerifyArgs
         const long long d = tokens[i];
         fine = false;
         if (d >= 0 && d < a.vocab) {
-          const double q = draft == nullptr ? 1.0 : (double)to_f32(draft[i * a.draft_row + d]);
+          const double q = draft == nullptr ? 1.0 : (double)clean(to_f32(draft[i * a.draft_row + d]));
           fine = (double)uniforms[i] * q < (double)to_f32(target[i * a.target_row + d]);
         }
       }

@@ -45,7 +45,8 @@ def attend(q, key_cache, value_cache, tables, lens, scale, shared_prefix=0):
 
 
 def verify(target, tokens, uniforms, draft=None, counts=None):
-    """(tokens [B, K + 1], accepted [B]) by the definition, one sequence and one column after the other."""
+    """(tokens [B, K + 1], accepted [B]) by the definition, one sequence and one column after the other. A probability that is
+    NaN or negative, the target's or the draft's, counts as 0."""
     b, rows, vocab = target.shape
     k = rows - 1
     out = torch.full((b, rows), -1, dtype=torch.int64)
@@ -62,19 +63,19 @@ def verify(target, tokens, uniforms, draft=None, counts=None):
             d = int(tokens[i, j])
             u = float(uniforms[i, j])
             inside = 0 <= d < vocab
-            q = 1.0 if draft is None else float(draft[i, j, d]) if inside else 0.0
-            if inside and u * q < float(target[i, j, d]):
+            q = 1.0 if draft is None else float(clean(draft[i, j, d])) if inside else 0.0
+            if inside and u * q < float(clean(target[i, j, d])):
                 out[i, j] = d
                 continue
-            p = target[i, j].double()
+            p = clean(target[i, j])
             if draft is None:
-                w = clean(p)
+                w = p.clone()
                 if inside:
                     w[d] = 0.0
             else:
-                w = clean(p - draft[i, j].double())
+                w = clean(p - clean(draft[i, j]))
             if not w.sum() > 0:
-                w = clean(p)
+                w = p
             a = j
             break
         accepted[i] = a

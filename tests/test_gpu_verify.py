@@ -141,3 +141,29 @@ def test_after_softmax_two_calls_streams_and_graphs():
     torch.cuda.synchronize()
     for got in (first, second, third, fourth):
         assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [40, 41, 4096])  # vectors, single elements, a step for each warp
+def test_draft_probabilities_that_are_nan_or_negative_count_as_zero(v, dtype):
+    """At the drafted token (which is then accepted wherever the target gives it anything) and beside it (where the column
+    keeps the target's own weight, no more and no less). Sums of eighths are exact."""
+    target = torch.zeros(8, 2, v, dtype=dtype)
+    target[:, :, 4], target[:, :, 9], target[:, :, v - 1] = 0.25, 0.25, 0.5
+    draft = torch.zeros(8, 1, v, dtype=dtype)
+    draft[:, 0, 4], draft[:, 0, 9], draft[:, 0, v - 1] = 0.125, 0.75, 0.125
+    bad = torch.tensor([float("nan"), -0.25, float("nan"), -1.0, float("nan"), -0.5, float("-inf"), float("nan")], dtype=dtype)
+    tokens = torch.full((8, 1), 9)
+    u = torch.tensor([[0.99, 0.3], [0.99, 0.3], [0.5, 0.3], [0.5, 0.3], [0.5, 0.45], [0.5, 0.45], [0.5, 0.45], [0.5, 0.9]])
+    draft[:2, 0, 9] = bad[:2]  # at the drafted token
+    draft[2:7, 0, 4] = bad[2:7]  # beside it: w = (0.25, 0, 0.375) of 0.625 in all, so 0.3 draws column 4 and 0.45 the last
+    draft[7, 0, :4] = bad[7]  # where the target has nothing
+    target[6, 0, 2] = -1.0  # below zero in both
+    draft[6, 0, 2] = -2.0
+    got = check(target, tokens, u, draft)
+    assert got[1].tolist() == [1, 1, 0, 0, 0, 0, 0, 0]
+    assert got[0][:, 0].tolist() == [9, 9, 4, 4, v - 1, v - 1, v - 1, v - 1]
+    p, t, u, q = problem(21, 6, 3, v, dtype)
+    q[:, :, ::3] = float("nan")
+    q[:, :, 1::3] *= -1.0
+    check(p, t, u, q)

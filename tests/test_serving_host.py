@@ -200,3 +200,16 @@ def test_the_oracle_of_the_verification_is_the_definition():
     assert serving.verify(target, tok, torch.tensor([[0.4, 0.4]]), draft)[0].tolist() == [[0, -1]]  # w = (.25, 0, .25)
     assert serving.verify(target, tok, torch.tensor([[0.4, 0.5]]), draft)[0].tolist() == [[2, -1]]
     assert serving.verify(target, tok, torch.tensor([[0.3, 0.4]]))[0].tolist() == [[0, -1]]  # one-hot: .3 >= .25
+
+
+def test_the_oracle_of_the_verification_takes_bad_probabilities_as_zero():
+    nan = float("nan")
+    target = torch.tensor([[[0.5, 0.25, 0.25], [0.0, 0.5, 0.5]]])
+    tok = torch.tensor([[1]])
+    for q in (nan, -0.5):
+        at = torch.tensor([[[0.25, q, 0.0]]])
+        assert serving.verify(target, tok, torch.tensor([[0.99, 0.4]]), at)[0].tolist() == [[1, 1]]  # as q = 0: accepted
+        beside = torch.tensor([[[q, 0.75, 0.25]]])  # refused; w = (.5, 0, 0)
+        assert serving.verify(target, tok, torch.tensor([[0.5, 0.9]]), beside)[0].tolist() == [[0, -1]]
+    target[0, 0, 2], less = -1.0, torch.tensor([[[0.0, 0.75, -2.0]]])  # w = (.5, 0, 0), not (.5, 0, 1)
+    assert serving.verify(target, tok, torch.tensor([[0.5, 0.9]]), less)[0].tolist() == [[0, -1]]
