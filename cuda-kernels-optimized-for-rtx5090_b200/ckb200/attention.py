@@ -54,8 +54,10 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     block_size, Hkv, D] in the same dtype; block_tables [B, M] int64, the blocks of each sequence in order; seq_lens [B]
     int64, the tokens of each sequence with the T new ones. Token t sees the positions below seq_lens - T + t + 1; with
     none (a padded row of the batch: length 0) its output is zeros. scale defaults to D ** -0.5. shared_prefix: the number
-    of tokens (a multiple of block_size) with which every sequence begins in the SAME blocks; they are read once, through
-    row 0 of block_tables. A block id outside the cache reads as zeros. Scores, softmax statistics and sums are fp32."""
+    of tokens (a multiple of block_size) with which the sequences begin in the SAME blocks; they are read once, through the
+    block_tables row of the first sequence all of whose T tokens see them all. Sequences that end before that (padded rows
+    among them) are read through their own rows, so a row's entries behind its length are never looked at. A block id
+    outside the cache reads as zeros. Scores, softmax statistics and sums are fp32."""
     problem = _problem(q, key_cache, value_cache, block_tables, seq_lens, shared_prefix)
     if problem:
         raise ValueError(f"attention: {problem}")

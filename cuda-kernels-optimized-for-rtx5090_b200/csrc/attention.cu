@@ -175,6 +175,17 @@ __device__ __forceinline__ long long length_of(const Args& a, int b) {
 __device__ __forceinline__ int own_begin(int prefix, int tokens, int len) {
   return len - tokens + 1 >= prefix ? prefix : 0;
 }
+// The first sequence that sees all of the prefix (0 where none does): its table names the shared blocks, as those of padded
+// rows and of shorter sequences may hold anything there. The whole warp asks.
+__device__ __forceinline__ int first_sharing(const Args& a) {
+  for (int base = 0; base < a.batch; base += 32) {
+    const int b = base + (threadIdx.x & 31);
+    const bool sees = b < a.batch && own_begin(a.prefix, a.tokens, (int)length_of(a, b)) > 0;
+    const unsigned some = __ballot_sync(0xffffffffu, sees);
+    if (some != 0u) return base + __ffs(some) - 1;
+  }
+  return 0;
+}
 
 // A place on the axis of tiles.
 struct Cursor {
@@ -352,13 +363,14 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
   if (!kShared && a.beside && blockIdx.x == 0 && first >= last) pdl_wait();
   if (first >= last) return;
 
+  const long long* shared_table = kShared ? a.tables + (long long)first_sharing(a) * a.table_width : nullptr;
   // The cache row of position (tile, lane of the tile), or -1.
   const auto lookup = [&](const Cursor& c, int i) -> long long {
     const int end = kShared ? a.prefix : cum[a.batch + 1 + c.b];
     const int pos = (kShared ? 0 : own_begin(a.prefix, a.tokens, end)) + c.tile * kTile + i;
     if (pos >= end) return -1;
     const int page = pos / a.block_size;
-    const long long block = __ldg(a.tables + (kShared ? 0LL : (long long)c.b * a.table_width) + page);
+    const long long block = __ldg((kShared ? shared_table : a.tables + (long long)c.b * a.table_width) + page);
     if (block < 0 || block >= a.num_blocks) return -1;
     return block * a.block_size + (pos - page * a.block_size);
   };

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int outside = (int)(a.num_blocks * a.block_size);  // rows of zeros, which a weight of zero must meet
     const bool leader = elect_one();
     // Lane p looks up page p of a tile a tile ahead, as in attend_stream.
+    const long long* table = a.tables;
     long long block_next = -1;
     int inside_next = 0;
     const auto look_up = [&](int tile) {
@@ -202,11 +203,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       if (lane >= pages || pos >= a.prefix) return;
       const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
       inside_next = pos - page * a.block_size;
-      block_next = __ldg(a.tables + page);
+      block_next = __ldg(table + page);
     };
     int unit = first / p.tiles, tile = first - unit * p.tiles;
     int in_piece = 0, uses0 = 0, uses1 = 0;
-    look_up(tile);
+    look_up(tile);  // through the first row, on its way while the lengths say whether that is the one to use
+    const int row = first_sharing(a);
+    if (row != 0) {
+      table += (long long)row * a.table_width;
+      look_up(tile);
+    }
     for (int w = first; w < last; ++w) {
       // Alternate tiles of a piece have a stage each, that of their group, so that every group meets its stage's phases
       // one after the other.

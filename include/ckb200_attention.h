@@ -21,7 +21,9 @@ long long ckb_attention_workspace(long long batch, int tokens, int q_heads, int 
  * included (clamped to [0, table_width * block_size]). Token t of sequence b sees the positions below lens[b] - tokens
  * + t + 1; out [batch, tokens, q_heads, head_dim] (contiguous) = softmax(scale * q . k) v over them, zeros where there
  * are none. q head h reads kv head h / (q_heads / kv_heads). shared_prefix: a multiple of block_size; the first
- * shared_prefix tokens are the same blocks for the whole batch and are read through row 0 of tables, once for all.
+ * shared_prefix tokens are the same blocks for the whole batch and are read once for all, through the row of tables of
+ * the first sequence all of whose new tokens see them (shorter ones, padded rows among them, through their own row: a
+ * row's entries behind its length are not looked at).
  * head_dim a multiple of 8, at most 256; batch at most 4096. work: the workspace (16-byte aligned, contents do not
  * matter before and after). No counterpart in the reference. */
 int ckb_attention_paged_launch(const void* q, const void* key_cache, const void* value_cache, const void* tables,

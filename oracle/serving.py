@@ -18,15 +18,18 @@ def norm_rotate(x, weight, cos, sin, eps):
 
 
 def attend(q, key_cache, value_cache, tables, lens, scale, shared_prefix=0):
-    """(out, the weighted mean of |v|) [B, T, Hq, D] in fp64. The first shared_prefix tokens come from row 0 of tables."""
+    """(out, the weighted mean of |v|) [B, T, Hq, D] in fp64. Where all T tokens of a sequence see shared_prefix tokens,
+    these come from the first such sequence's row of tables."""
     b, t, hq, d = q.shape
     block_size, hkv = key_cache.shape[1:3]
     out = torch.zeros(q.shape, dtype=torch.float64)
     size = torch.zeros(q.shape, dtype=torch.float64)
     shared = shared_prefix // block_size
+    lengths = [max(0, min(int(n), tables.shape[1] * block_size)) for n in lens]
+    sharing = [i for i in range(b) if lengths[i] - t + 1 >= shared_prefix]
     for i in range(b):
-        ids = torch.cat([tables[0, :shared], tables[i, shared:]])
-        length = max(0, min(int(lens[i]), ids.numel() * block_size))
+        ids = torch.cat([tables[sharing[0] if i in sharing else i, :shared], tables[i, shared:]])
+        length = lengths[i]
         ids = ids[: -(-length // block_size)]
         fine = (ids >= 0) & (ids < key_cache.shape[0])
         at = ids.clamp(0, key_cache.shape[0] - 1)

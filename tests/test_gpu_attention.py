@@ -351,3 +351,18 @@ def test_a_drafted_decoding_step():
     graph.replay()
     torch.cuda.synchronize()
     assert bits_equal(got[1], out) and torch.equal(got[3], tokens)
+
+
+@pytest.mark.parametrize("d,bs", [(128, 16), (64, 8), (64, 24), (256, 16)])  # tcgen05 with boxes of 16 and 8 rows; copies
+@pytest.mark.parametrize("before", [1, 40])  # within and beyond the first 32 sequences
+def test_the_prefix_is_found_behind_padded_rows_and_short_sequences(d, bs, before):
+    """The rows in front are padding or end inside the prefix, and what their tables hold behind their lengths is anything."""
+    lens = [0] * (before - 1) + [bs + 1, 4 * bs + 5, 4 * bs, 4 * bs + 70]  # with two tokens each, 4 bs is one too short
+    q, kc, vc, tables, lens = problem(24 + before, BF, 2, 4, 2, d, bs, lens, 4 * bs)
+    want = check(q, kc, vc, tables, lens, 4 * bs)
+    for i, n in enumerate(lens.tolist()):
+        tables[i, -(-n // bs):] = torch.tensor([-1, 1 << 40, kc.shape[0]])[i % 3]
+    assert bits_equal(check(q, kc, vc, tables, lens, 4 * bs), want)
+    tables[:, :4] = tables[before, :4]  # nobody sees it all: the tables' first rows are not used for others either
+    tables[0] = -1
+    check(q, kc, vc, tables, lens.clamp_max(4 * bs), 4 * bs)
