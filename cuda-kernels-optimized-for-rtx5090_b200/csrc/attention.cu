@@ -5,7 +5,9 @@
 // computed piece by piece: a piece of positions gives (m, l = sum exp(x - m), o = sum exp(x - m) v), and pieces join by
 //   M = max m_i,  out = sum_i exp(m_i - M) o_i / sum_i exp(m_i - M) l_i.
 // x, m, l and o are fp32; the weights exp(x - m) are rounded to the cache's dtype for the product with v (half a step of
-// that dtype on each, as the output's own rounding), q, k and v enter the products as they are.
+// that dtype on each, as the output's own rounding), q, k and v enter the products as they are. fp16 has no half step of a
+// small value: below 2^-14 its steps stay 2^-24, and a weight below 2^-25 would be lost, of which a long context has many.
+// So its weights are exp(x - m) 2^15 (weights_from); any m will do for a piece, as long as l, o and the join take the same.
 //
 // Two kinds of work:
 //   own     the positions behind the prefix: a unit is (sequence, kv head, up to 64 of its T * group rows), its tiles are 64
@@ -44,6 +46,8 @@ constexpr int kPrefixRun = 4;
 constexpr int kPrefixCtaNs = 9000, kPrefixTileNs = 1900, kOwnTileNs = 2000;
 constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
+// The power of 2 by which fp16 weights are lifted: at most 2^15 then, and half a step of the smallest is 2^-40 of the largest.
+constexpr float kLift = 15.0f;
 
 struct View3 {
   long long batch, token, head;
@@ -116,6 +120,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// What is taken off a row's scores (in powers of 2) whose maximum is m, -inf where it has seen nothing: m, and for fp16
+// weights `lift` less. Beyond 2^20, where the rounding of m itself would show in the weights, they are not lifted.
+template <typename T>
+__device__ __forceinline__ float weights_from(float m, float lift) {
+  return std::is_same<T, __half>::value && fabsf(m) < 0x1p20f ? m - lift : m;
 }
 
 // Byte offset of 16-byte chunk c of row r in a tile of rows of DT 16-bit values: chunks are exchanged within a row so that
@@ -497,8 +508,9 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
       for (int n = 0; n < kNt; ++n) top = fmaxf(top, fmaxf(s[n][2 * i], s[n][2 * i + 1]) * a.scale_log2);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float ref = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet: exp2(-inf - 0) = 0
-      scale_o[i] = exp2_fast(m[i] - ref);
+      const float from = weights_from<T>(top, kLift);
+      const float ref = from == -INFINITY ? 0.0f : from;  // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      scale_o[i] = exp2_fast(weights_from<T>(m[i], kLift) - ref);
       m[i] = top;
       float sum = 0.0f;
 #pragma unroll
@@ -561,6 +573,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        m[i] = weights_from<T>(m[i], kLift);
       }
       if (S::kKeyWarps > 1) {  // join the warps that shared the positions, in the tile's own stage
         if ((lane & 3) == 0) {

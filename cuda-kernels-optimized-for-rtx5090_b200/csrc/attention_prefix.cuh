@@ -15,7 +15,8 @@
 // which lies over S, had to be used up first.)
 // The two groups have a row tile of 128 each of a 256-row unit, or every other tile of positions of a 128-row unit (then
 // they are two pieces). O stays in TMEM. It is scaled down only when a row's maximum has risen by more than 8 (powers of
-// 2) over the one in use; until then weights may reach 2^8, which fp32 sums and 16-bit weights hold as well as 1.
+// 2) over the one in use; until then weights may reach 2^8, which fp32 sums and 16-bit weights hold as well as 1. (fp16
+// weights are lifted by 7 then, and reach 2^15.)
 // 1024 rows x 8 heads x 16384 positions at D = 128 take 79 us, 870 TFLOP/s or 0.51 of the measured matrix rate, the tensor
 // cores busy 43 % of the time. A step of the two groups takes 1500 clocks: products of 64 columns take 55 clocks instead of
 // the 32 of their operations (both operands come from shared memory), 1420 in all for a step of the two; 128 columns have no
@@ -30,6 +31,7 @@ constexpr int kGroupRows = 128;   // query rows of a softmax group
 constexpr int kPrefixThreads = 384;
 constexpr int kStep = 64;         // positions of a step
 constexpr float kSlack = 8.0f;    // by how much a maximum may fall behind
+constexpr float kPrefixLift = kLift - kSlack;
 
 // ---------------------------------------------------------------------------------------------------------------
 // tcgen05 and TMEM, against the PTX ISA for sm_100a.
@@ -340,7 +342,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         mbar_arrive(&q_full[g]);
       }
 
-      float m = -INFINITY, l = 0.0f;
+      constexpr float kHighest = std::is_same<T, __half>::value ? kLift : kSlack;  // of a score over m
+      float m = -INFINITY, l = 0.0f;  // m: what is taken off the scores
       const int steps = !alternate ? 2 * count : g == 0 ? (count + 1) / 2 * 2 : count / 2 * 2;
       for (int u = 0; u < steps; ++u, ++step) {
         const int buffer = step & 1, tile = tile0 + (alternate ? (u & ~1) + g : u >> 1);
@@ -368,9 +371,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           top[(e >> 1) & 3] = max3(top[(e >> 1) & 3], __uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
         if (u == 0) {
-          m = most;
-        } else if (__any_sync(0xffffffffu, most > m + kSlack)) {
-          const float rise = fmaxf(m, most), down = exp2_fast(m - (rise == -INFINITY ? 0.0f : rise));
+          m = weights_from<T>(most, kPrefixLift);
+        } else if (__any_sync(0xffffffffu, most > m + kHighest)) {
+          const float rise = fmaxf(m, weights_from<T>(most, kPrefixLift)), down = exp2_fast(m - (rise == -INFINITY ? 0.0f : rise));
           m = rise;
           l *= down;
           // The last step's product has reached O (the one before it had, or these scores would not be there).

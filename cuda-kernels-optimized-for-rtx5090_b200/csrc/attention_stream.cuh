@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {  // a new maximum: rarer and rarer along the tiles
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float scale = exp2_fast(m[i] - (top[i] == -INFINITY ? 0.0f : top[i]));
+        const float from = weights_from<T>(top[i], kLift);
+        const float scale = exp2_fast(weights_from<T>(m[i], kLift) - (from == -INFINITY ? 0.0f : from));
         m[i] = top[i];
         l[i] *= scale;
 #pragma unroll
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float ref = m[i] == -INFINITY ? 0.0f : m[i];  // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      const float from = weights_from<T>(m[i], kLift);
+      const float ref = from == -INFINITY ? 0.0f : from;  // a row that has seen nothing yet: exp2(-inf - 0) = 0
       float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < kNt; ++n)
@@ -378,6 +380,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        m[i] = weights_from<T>(m[i], kLift);
       }
       if (S::kKeyWarps == 1) {
 #pragma unroll

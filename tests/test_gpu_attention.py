@@ -366,3 +366,43 @@ def test_the_prefix_is_found_behind_padded_rows_and_short_sequences(d, bs, befor
     tables[:, :4] = tables[before, :4]  # nobody sees it all: the tables' first rows are not used for others either
     tables[0] = -1
     check(q, kc, vc, tables, lens.clamp_max(4 * bs), 4 * bs)
+
+
+@pytest.mark.parametrize("bs", [16, 24])
+@pytest.mark.parametrize("prefix,sink", [(0, 0), (0, 2000), (16320, 5), (16320, 8000)])
+def test_many_small_weights_beside_a_large_one(prefix, sink, bs):
+    """One position takes nearly all the weight and thousands have 2^-26 of it each, which is less than half of fp16's
+    smallest step, but 0.00006 and more together: all that the output is made of where the large one's value is zero. Heads
+    and sequences enough that a CTA meets many of the positions in one piece.
+    The bound is assert_near's, with the small weights off by half of 2^-24 of a weight that is lifted by 2^15, or by 2^7
+    where that is all that the shared work does: n 2^-32 of the largest |v|, not n 2^-25."""
+    prefix, heads = prefix // bs * bs, 16
+    n = prefix + 41 if prefix else 4000
+    q, kc, vc, tables, lens = problem(25, HF, 1, heads, heads, 64, bs, [n] * (2 if prefix else 24), prefix)
+    q.fill_(1.0)
+    kc[kc.isfinite()] = 0.0
+    vc[:] = vc.abs() + 0.5
+    rows = tables[:, sink // bs] * bs + sink % bs
+    kc.view(-1, heads, 64)[rows] = 2.25  # a score of 64 * 2.25 / 8 = 18: exp(-18) = 2^-25.97
+    vc.view(-1, heads, 64)[rows] = 0.0
+    got = attention.paged_attention(*(t.cuda() for t in (q, kc, vc, tables, lens)), shared_prefix=prefix).cpu().double()
+    want, size = serving.attend(q, kc, vc, tables, lens, 64 ** -0.5, prefix)
+    v = vc[vc.isfinite()].double().abs().max().item()
+    bound = 2.0 ** -11 * (want.abs() + size) + 2 * size * ((64 / 16 + 20) * 2.0 ** -23 * 18 + 2.0 ** -18) + n * 2.0 ** -32 * v + 2.0 ** -25
+    assert (want > 2.0 ** -15).all() and ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("prefix", [0, 512])
+@pytest.mark.parametrize("shift", [-3e5, 3e5, 1.5e6, -1.5e6])  # to either side of 2^20 in powers of 2
+def test_scores_far_from_zero(shift, prefix, dtype):
+    """All scores of a row share a large term; what fp32 leaves of their differences has to come out as finite weights that
+    add up: with values of 1 the output is 1, but for half a step of the weights and of itself, 2^-18 of the sums and, where
+    fp16 weights are not lifted, 2^-25 for each of the 612."""
+    q, kc, vc, tables, lens = problem(26, dtype, 1, 2, 1, 64, 16, [512 + 100, 512 + 30], prefix)
+    q = 0.5 * torch.randn(q.shape, generator=torch.Generator().manual_seed(27)).to(dtype)
+    q[..., 0], seen = 1024.0, kc.isfinite()
+    kc[..., 0] = torch.where(seen[..., 0], shift * 8 / 1024 / 64, kc[..., 0])  # scale 64 / 8: shift in all
+    vc[vc.isfinite()] = 1.0
+    got = attention.paged_attention(*(t.cuda() for t in (q, kc, vc, tables, lens)), scale=8.0, shared_prefix=prefix)
+    assert ((got.cpu().double() - 1).abs() <= torch.finfo(dtype).eps + 2.0 ** -18 + 612 * 2.0 ** -25).all()
