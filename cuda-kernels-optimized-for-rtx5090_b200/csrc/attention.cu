@@ -177,8 +177,13 @@ __device__ __forceinline__ Row row_of(const Args& a, int b, int kv_head, int r) 
   x.head = kv_head * a.group + (in - x.t * a.group);
   return x;
 }
+// The lengths and tables. The own work beside a prefix starts without a wait of its own (start_all): what came before on the
+// stream has ended, as the shared work's CTAs waited for it before they let it start, but only a grid's own wait is said to
+// make it visible to that grid. So all its inputs are read in L2, past an SM's L1, where an older copy could lie: these two
+// lists here, the queries by cp.async.cg, the cache by TMA or cp.async.cg.
+__device__ __forceinline__ long long load_list(const long long* p) { return __ldcg(p); }
 __device__ __forceinline__ long long length_of(const Args& a, int b) {
-  const long long most = (long long)a.table_width * a.block_size, n = __ldg(a.lens + b);
+  const long long most = (long long)a.table_width * a.block_size, n = load_list(a.lens + b);
   return n < 0 ? 0 : n < most ? n : most;
 }
 // Where a sequence's own positions begin: behind the prefix, or, for one that does not see all of it, at 0: such a sequence
@@ -381,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) attend_tiles(const Args a) {
     const int pos = (kShared ? 0 : own_begin(a.prefix, a.tokens, end)) + c.tile * kTile + i;
     if (pos >= end) return -1;
     const int page = pos / a.block_size;
-    const long long block = __ldg((kShared ? shared_table : a.tables + (long long)c.b * a.table_width) + page);
+    const long long block = load_list((kShared ? shared_table : a.tables + (long long)c.b * a.table_width) + page);
     if (block < 0 || block >= a.num_blocks) return -1;
     return block * a.block_size + (pos - page * a.block_size);
   };

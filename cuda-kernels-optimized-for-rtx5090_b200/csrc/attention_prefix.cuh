@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       if (lane >= pages || pos >= a.prefix) return;
       const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
       inside_next = pos - page * a.block_size;
-      block_next = __ldg(table + page);
+      block_next = load_list(table + page);
     };
     int unit = first / p.tiles, tile = first - unit * p.tiles;
     int in_piece = 0, uses0 = 0, uses1 = 0;

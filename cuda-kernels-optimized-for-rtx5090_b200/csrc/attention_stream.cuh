@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
       if (!there_next) return;
       const int page = a.block_log >= 0 ? pos >> a.block_log : pos / a.block_size;
       inside_next = pos - page * a.block_size;
-      block_next = __ldg(a.tables + (long long)c.b * a.table_width + page);
+      block_next = load_list(a.tables + (long long)c.b * a.table_width + page);
     };
     int q_loads = 0, stage = 0, parity = 1;
     look_up(at);

@@ -406,3 +406,61 @@ def test_scores_far_from_zero(shift, prefix, dtype):
     vc[vc.isfinite()] = 1.0
     got = attention.paged_attention(*(t.cuda() for t in (q, kc, vc, tables, lens)), scale=8.0, shared_prefix=prefix)
     assert ((got.cpu().double() - 1).abs() <= torch.finfo(dtype).eps + 2.0 ** -18 + 612 * 2.0 ** -25).all()
+
+
+def test_inputs_that_the_kernel_just_before_wrote():
+    """Lengths and tables moved on in place, and the cache written by qk_norm_rope_kv_cache, right before each call behind a
+    shared prefix, with no synchronisation: the bits of the same steps with one after each. Steps of 3 tokens over 40 rounds,
+    eagerly and as a replayed graph; the tables are turned between two sets of pages that hold different tokens."""
+    b, t, hq, hkv, d, bs, prefix, rounds = 24, 3, 8, 2, 64, 16, 128, 40
+    g = torch.Generator().manual_seed(28)
+    start = [prefix + 3 + 5 * i for i in range(b)]
+    q, kc, vc, tables, lens = problem(28, BF, t, hq, hkv, d, bs, start, prefix, spare=10)
+    kc, vc = (torch.randn(2 * c.shape[0], *c.shape[1:], generator=g).to(BF) for c in (kc, vc))  # pages of the other set
+    shift = torch.zeros_like(tables)
+    shift[:, prefix // bs:] = kc.shape[0] // 2
+    qkv = torch.randn(rounds, b, t, (hq + 2 * hkv) * d, generator=g).to(BF).cuda()
+    cos, sin = (c.cuda() for c in orope.cos_sin_cache(10000.0, d, 1024))
+    w = torch.ones(d, device="cuda")
+    first = [x.cuda() for x in (kc, vc, tables, lens)]
+    shift, step_ids = shift.cuda(), torch.arange(t, device="cuda") - t
+
+    def run(sync, graph=None):
+        state = [x.clone() for x in first]
+        kc, vc, tables, lens = state
+        sign, now, x = torch.ones((), dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"), None
+        outs = []
+
+        def step():
+            ids = lens[:, None] + t + step_ids
+            slots = torch.gather(tables + sign * shift, 1, ids // bs) * bs + ids % bs
+            parts = qkv[now][0].split([hq * d, hkv * d, hkv * d], -1)
+            q, k, v = (p.unflatten(-1, (-1, d)) for p in parts)
+            now.add_(1)
+            tables.add_(sign * shift)
+            sign.neg_()
+            lens.add_(t)
+            q, _ = rope.qk_norm_rope_kv_cache(q, k, v, ids, w, w, cos, sin, kc, vc, slots, inplace=False, write_k=False)
+            return attention.paged_attention(q, kc, vc, tables, lens, shared_prefix=prefix)
+
+        if graph is not None:
+            with torch.cuda.graph(graph):
+                x = step()
+        for _ in range(rounds):
+            if graph is None:
+                outs.append(step())
+            else:
+                graph.replay()
+                outs.append(x.clone())
+            if sync:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs, state
+
+    want, kept = run(True)
+    for _ in range(3):
+        got, state = run(False)
+        assert all(bits_equal(x, y) for x, y in zip(got, want))
+        assert all(torch.equal(x, y) for x, y in zip(state[2:], kept[2:]))
+    got, _ = run(False, torch.cuda.CUDAGraph())
+    assert all(bits_equal(x, y) for x, y in zip(got, want))
