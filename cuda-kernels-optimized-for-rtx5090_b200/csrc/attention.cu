@@ -24,6 +24,7 @@
 #include "ckb200_attention.h"
 #include "common.cuh"
 
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -37,7 +38,9 @@ constexpr int kSmShared = 233472;   // and an SM has
 // The shared work takes at most 7 of 8 SMs, so that own tokens are read from its first moment on (256 sequences behind 16384
 // tokens 128 us, with 6 of 8 SMs 131 us, with all 135 us), and runs of at least 4 tiles, as a CTA spends 5 us before its
 // first tile and 3 us on its piece (64 sequences behind 4096 tokens with up to 1023, up to 32 own tokens: 42 and 21 us; runs of 3
-// tiles 45 and 25 us, of 8 tiles 41 and 27 us).
+// tiles 45 and 25 us, of 8 tiles 41 and 27 us). Where units are shorter than that and many, a run has several of them: 256
+// sequences of 5 tokens with 20 rows a key head behind 128 tokens took 138 us with a CTA for each of the 160 units, 126 us with two
+// units a CTA; 512 of 4 tokens with 256 units 154 us and 159 us.
 constexpr int kPrefixShare = 7;
 constexpr int kPrefixRun = 4;
 // What the shared work's CTAs are expected to take: 9 us and 1.9 us a tile (half where its groups share the tiles). The own
@@ -831,7 +834,7 @@ bool sizes_of(long long batch, int tokens, int q_heads, int kv_heads, int head_d
     const long long all = (long long)h.tiles * kv_heads * h.row_tiles;
     if (all > INT_MAX / 2) return false;
     h.run = (int)((all + at_once - 1) / at_once);
-    if (i == 0 && h.run < kPrefixRun) h.run = kPrefixRun < h.tiles ? kPrefixRun : h.tiles;
+    if (i == 0) h.run = std::max(h.run, std::min(kPrefixRun, h.tiles));  // longer than a short unit where units are many
     h.ctas = (int)((all + h.run - 1) / h.run);
     const long long need = ((long long)kv_heads * h.row_tiles + h.ctas) * h.slots * h.rows;
     if (need > shared_rows) shared_rows = need;

@@ -464,3 +464,10 @@ def test_inputs_that_the_kernel_just_before_wrote():
         assert all(torch.equal(x, y) for x, y in zip(state[2:], kept[2:]))
     got, _ = run(False, torch.cuda.CUDAGraph())
     assert all(bits_equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("t,heads,lens", [(1, 320, [129, 140]), (1, 150, [128 + i % 20 for i in range(130)])])
+@pytest.mark.parametrize("prefix", [128, 112])
+def test_short_prefixes_of_more_units_than_ctas(t, heads, lens, prefix):
+    """A CTA has several units of one tile one after the other: of 2 rows, and of 130."""
+    check(*problem(29, BF, t, heads, heads, 64, 16, lens, prefix), prefix)

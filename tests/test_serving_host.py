@@ -213,3 +213,17 @@ def test_the_oracle_of_the_verification_takes_bad_probabilities_as_zero():
         assert serving.verify(target, tok, torch.tensor([[0.5, 0.9]]), beside)[0].tolist() == [[0, -1]]
     target[0, 0, 2], less = -1.0, torch.tensor([[[0.0, 0.75, -2.0]]])  # w = (.5, 0, 0), not (.5, 0, 1)
     assert serving.verify(target, tok, torch.tensor([[0.5, 0.9]]), less)[0].tolist() == [[0, -1]]
+
+
+@pytest.mark.parametrize("prefix", [128, 256, 384, 512, 4096])
+@pytest.mark.parametrize("batch,tokens,q_heads,kv_heads", [(640, 4, 32, 8), (2, 1, 160, 160), (2, 1, 400, 400), (256, 5, 32, 8),
+                                                           (64, 1, 32, 8), (16, 1, 8, 2), (1000, 8, 64, 8)])
+def test_the_shared_work_leaves_an_eighth_of_the_sms(batch, tokens, q_heads, kv_heads, prefix):
+    """Its pieces' part of the workspace is 2 x 128 rows (a row: D sums and two statistics) for each unit and each CTA, or what
+    the form without tensor memory needs where that is more: so it bounds the CTAs, of which 7 for 8 of the 148 SMs are allowed."""
+    lib = _native.load("attention")
+    size = [lib.ckb_attention_workspace(batch, tokens, q_heads, kv_heads, 128, 16, 1024, n) for n in (prefix, 0)]
+    rows = (size[0] - size[1]) // (128 * 4 + 8)
+    all_rows = batch * tokens * (q_heads // kv_heads)
+    units = kv_heads * -(-all_rows // (256 if all_rows > 128 else 128))
+    assert 0 < rows and rows / 256 - units < 148 * 7 // 8 + 1
