@@ -1078,7 +1078,8 @@ CKB_EXPORT int ckb_attention_paged_launch(const void* q, const void* key_cache, 
 // Status of the bounded waits since the last reset: 0, or 1 when a wait gave up (that launch's output is void).
 CKB_EXPORT int ckb_attention_status(int reset) {
   unsigned int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();  // the copy alone does not wait for streams that are non-blocking
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(v));
   if (e != cudaSuccess) return -(int)e;
   if (reset && v != 0u) {
     const unsigned int zero = 0u;

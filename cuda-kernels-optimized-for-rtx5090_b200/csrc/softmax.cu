@@ -998,7 +998,8 @@ CKB_EXPORT int launch(const void* x, void* y, long long rows, long long cols, in
 // (the launch then produced garbage instead of hanging). Synchronises with the device; reset != 0 clears the word.
 CKB_EXPORT int ckb_softmax_status(int reset) {
   unsigned v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_softmax_status, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();  // the copy alone does not wait for streams that are non-blocking
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_softmax_status, sizeof(v));
   if (e != cudaSuccess) return -(int)e;
   if (reset) {
     const unsigned zero = 0;

@@ -1551,7 +1551,8 @@ CKB_EXPORT int ckb_topk_trace(void* out, int rows) {
 // vocab-sharded variant over peer memory) ran out. Synchronises with the device; reset != 0 clears the word.
 CKB_EXPORT int ckb_topk_status(int reset) {
   unsigned v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_topk_status, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();  // the copy alone does not wait for streams that are non-blocking
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_topk_status, sizeof(v));
   if (e != cudaSuccess) return -(int)e;
   if (reset) {
     const unsigned zero = 0;

@@ -471,3 +471,19 @@ def test_inputs_that_the_kernel_just_before_wrote():
 def test_short_prefixes_of_more_units_than_ctas(t, heads, lens, prefix):
     """A CTA has several units of one tile one after the other: of 2 rows, and of 130."""
     check(*problem(29, BF, t, heads, heads, 64, 16, lens, prefix), prefix)
+
+
+@pytest.mark.parametrize("op", ["attention", "softmax", "topk"])
+def test_reading_the_status_waits_for_every_stream(op):
+    """torch's streams are non-blocking: a copy on the legacy stream does not wait for them, the status has to."""
+    from ckb200 import _native
+
+    status = getattr(_native.load(op), f"ckb_{op}_status")
+    assert status(0) == 0  # a first call waits for everything anyway, while the library is loaded
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # 0.2 s at 2 GHz
+        done.record()
+    assert not done.query()
+    assert status(0) == 0
+    assert done.query()
