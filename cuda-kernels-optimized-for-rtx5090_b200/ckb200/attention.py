@@ -103,6 +103,22 @@ def paged_attention(q, key_cache, value_cache, block_tables, seq_lens, scale=Non
     return out
 
 
+def check(device=None):
+    """Synchronises the device (by default the current one) and raises RuntimeError when a wait of these kernels on a copy or a
+    product has run out there since the last check: every wait ends after 2 s at most, and outputs of the calls since then
+    may be void."""
+    lib = _native.load("attention")
+    if device is None:
+        status = lib.ckb_attention_status(1)
+    else:
+        with torch.cuda.device(device):
+            status = lib.ckb_attention_status(1)
+    if status < 0:
+        raise RuntimeError(f"attention: status read failed: CUDA error {-status}")
+    if status:
+        raise RuntimeError("attention: a wait inside a kernel ran out (2 s); the outputs since the last check may be void")
+
+
 def run(inputs):
     return {"out": paged_attention(inputs["q"], inputs["key_cache"], inputs["value_cache"], inputs["block_tables"],
                                    inputs["seq_lens"], inputs.get("scale"), inputs.get("shared_prefix", 0))}

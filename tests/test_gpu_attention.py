@@ -487,3 +487,10 @@ def test_reading_the_status_waits_for_every_stream(op):
     assert not done.query()
     assert status(0) == 0
     assert done.query()
+
+
+def test_check_passes_on_either_device_argument():
+    p = [t.cuda() for t in problem(30, BF, 1, 4, 2, 64, 16, [100, 70], 32)]
+    attention.paged_attention(*p, shared_prefix=32)
+    attention.check()
+    attention.check("cuda:0")

@@ -227,3 +227,24 @@ def test_the_shared_work_leaves_an_eighth_of_the_sms(batch, tokens, q_heads, kv_
     all_rows = batch * tokens * (q_heads // kv_heads)
     units = kv_heads * -(-all_rows // (256 if all_rows > 128 else 128))
     assert 0 < rows and rows / 256 - units < 148 * 7 // 8 + 1
+
+
+def test_a_wait_that_ran_out_is_raised(monkeypatch):
+    class Lib:
+        status = 0
+
+        def ckb_attention_status(self, reset):
+            assert reset == 1
+            status, self.status = self.status, 0
+            return status
+
+    lib = Lib()
+    monkeypatch.setattr(_native, "load", lambda op: lib)
+    attention.check()
+    lib.status = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        attention.check()
+    attention.check()
+    lib.status = -700
+    with pytest.raises(RuntimeError, match="CUDA error 700"):
+        attention.check()
