@@ -494,3 +494,38 @@ def test_check_passes_on_either_device_argument():
     attention.paged_attention(*p, shared_prefix=32)
     attention.check()
     attention.check("cuda:0")
+
+
+@pytest.mark.parametrize("bs", [16, 24])  # a TMA box for each page, and copies of 16 bytes
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [1, 5, 10, 20])  # 4, 20, 40 and 80 rows a key head: 1, 2 and 4 warps share the rows, or two row tiles
+def test_own_tokens_in_every_form(t, d, bs):
+    dtype = (BF, HF)[(t + d // 64) % 2]
+    check(*problem(31 + t, dtype, t, 8, 2, d, bs, [300, t - 1, 9, 0, 64, 700]))
+
+
+@pytest.mark.parametrize("bs", [24, 48, 7])  # no box fits a page
+@pytest.mark.parametrize("d", [64, 120, 128, 200])
+@pytest.mark.parametrize("dtype,t,group,count", [(BF, 2, 4, 20), (HF, 1, 1, 9), (HF, 1, 8, 8), (BF, 7, 4, 5)])  # 160, 9, 64, 140 rows
+def test_shared_prefix_without_boxes(dtype, t, group, count, d, bs):
+    prefix = {24: 168, 48: 336, 7: 133}[bs]
+    lens = [prefix + t + 3 * i for i in range(count)] + [prefix - 3, 0, 10, prefix + t - 1]
+    check(*problem(32 + d, dtype, t, 2 * group, 2, d, bs, lens, prefix), prefix)
+
+
+@pytest.mark.parametrize("bs", [16, 24])
+@pytest.mark.parametrize("group", [4, 8, 16])  # 16, 32 and 64 rows a key head
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("shared", [False, True])
+def test_values_that_a_row_must_not_see_in_every_form(shared, d, group, bs):
+    prefix = 4 * bs if shared else 0
+    q, kc, vc, tables, lens = problem(33 + d, (BF, HF)[group // 8 % 2], 4, 2 * group, 2, d, bs, [prefix + 130, prefix + 9], prefix)
+    check(q, kc, vc, tables, lens, prefix)
+    for b, n in enumerate(lens.tolist()):
+        block, at = tables[b, (n - 2) // bs], (n - 2) % bs  # seen by tokens 2 and 3
+        vc[block, at, 0, 3], kc[block, at, 1, 5] = float("inf"), float("nan")
+    # Tokens 0 and 1 by assert_near's bound, not by bits: the tile that holds the value is then summed one position after the
+    # other, not 16 at a time, and two fp32 sums that are each within 2^-18 of the exact one may round to either neighbour.
+    got = check(q, kc, vc, tables, lens, prefix)
+    assert got[:, :2].isfinite().all()
+    assert not got[:, 2:, :group, 3].isfinite().any() and got[:, 2:, group:].isnan().all()
