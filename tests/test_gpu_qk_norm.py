@@ -158,3 +158,20 @@ def test_other_stream_and_graph_replay():
     graph.replay()
     torch.cuda.synchronize()
     assert bits_equal(got[0], want2[0]) and bits_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("d,layout", [(128, "fused"), (40, "plain")])  # the vector and the scalar form
+def test_sincos_mode_with_the_cache_write(d, layout):
+    """theta in place of the cos/sin cache: the caches get what the call without them gives."""
+    g = torch.Generator().manual_seed(9)
+    q, k, v = heads(layout, g, torch.bfloat16, 3, 21, 8, 2, d)
+    w = (1 + 0.1 * torch.randn(d, generator=g)).cuda()
+    ids = torch.randint(0, 1 << 17, (3, 21), generator=g).cuda()
+    slots = torch.randperm(80, generator=g)[:63].view(3, 21).cuda()
+    caches = [torch.zeros(5, 16, 2, d, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    want_q, want_k = rope.qk_norm_rope(q, k, ids, w, w, theta=5e5)
+    got_q, got_k = rope.qk_norm_rope_kv_cache(q, k, v, ids, w, w, None, None, *caches, slots, theta=5e5, inplace=False)
+    assert bits_equal(got_q, want_q) and bits_equal(got_k, want_k)
+    for cache, new in zip(caches, (want_k, v)):
+        assert bits_equal(cache.view(-1, 2, d)[slots.flatten()], new.reshape(-1, 2, d))
+        assert (cache.view(-1, 2, d).abs().amax((1, 2)) > 0).sum() == 63
