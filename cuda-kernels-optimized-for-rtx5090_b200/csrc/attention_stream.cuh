@@ -103,8 +103,10 @@ struct Ring {
   static constexpr int bytes(int batch) { return kOffCum + (2 * batch + 1) * 4; }
   // CTAs of an SM by registers (with two stages of 32 KB each three CTAs keep as many bytes in flight as two with three
   // stages, and 12 warps multiply instead of 8: 64 sequences behind 4096 tokens 45.6 -> 42.0 us, 48 ragged ones 259 -> 252;
-  // one of 8192 tokens, whose CTAs have an SM for themselves, 11.9 -> 13.1).
-  static constexpr int kPerSm = DT <= 64 ? 4 : DT <= 128 ? (WR == 1 ? 3 : 2) : 1;
+  // one of 8192 tokens, whose CTAs have an SM for themselves, 11.9 -> 13.1). Of heads of 64 columns four, with up to 32 rows; 64
+  // rows spill at the 96 registers of four (32 sequences of 16 tokens, 4 heads a key head, behind 1024 tokens 93 us, with three 69 us; 48
+  // ragged ones without a prefix 158 and 151 us).
+  static constexpr int kPerSm = DT <= 64 ? (WR == 4 ? 3 : 4) : DT <= 128 ? (WR == 1 ? 3 : 2) : 1;
   // ... and by shared memory, of which the system takes 1 KB for each.
   static int per_sm(int batch) {
     const int fit = kSmShared / (bytes(batch) + 1024);
