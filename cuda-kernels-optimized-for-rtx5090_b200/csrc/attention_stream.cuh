@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     v_row[n] = row_part<DT>(wk * kKeys + n * 16 + (lane & 15), rows_log);
   }
   constexpr int kNt = kKeys / 8, kDt = DT / 8;
-  float o[kDt][4], m[2], l[2];
+  constexpr bool kLifted = std::is_same<T, __half>::value;
+  float o[kDt][4], m[2], l[2], from[2];  // from: weights_from of m, where that is another
   int len = 0, begin = 0, min_limit = 0, lim[2] = {0, 0}, q_now = -1, piece_begin = 0, stage = 0, parity = 0;
   for (int w = first; w < last; ++w) {
     const int kv_head = a.row_tiles == 1 ? at.unit : at.unit / a.row_tiles, row0 = (at.unit - kv_head * a.row_tiles) * kRows;
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
         const int in = row0 + wr * 16 + quad_row + 8 * i;
         lim[i] = in < a.rows ? max(0, len - a.tokens + in / a.group + 1) : INT_MAX;  // padding: any finite result
         m[i] = -INFINITY;
+        if constexpr (kLifted) from[i] = -INFINITY;
         l[i] = 0.0f;
       }
       min_limit = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));
@@ -299,9 +301,10 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {  // a new maximum: rarer and rarer along the tiles
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float from = weights_from<T>(top[i], kLift);
-        const float scale = exp2_fast(weights_from<T>(m[i], kLift) - (from == -INFINITY ? 0.0f : from));
+        const float next = weights_from<T>(top[i], kLift);
+        const float scale = exp2_fast((kLifted ? from[i] : m[i]) - (next == -INFINITY ? 0.0f : next));
         m[i] = top[i];
+        if constexpr (kLifted) from[i] = next;
         l[i] *= scale;
 #pragma unroll
         for (int n = 0; n < kDt; ++n) {
@@ -312,8 +315,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float from = weights_from<T>(m[i], kLift);
-      const float ref = from == -INFINITY ? 0.0f : from;  // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      const float ref = m[i] == -INFINITY ? 0.0f : kLifted ? from[i] : m[i];  // a row that has seen nothing yet: exp2(-inf - 0) = 0
       float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < kNt; ++n)
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(32 * (kConsumers + 1), Ring<DT, WR>::kPerSm)
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        m[i] = weights_from<T>(m[i], kLift);
+        if constexpr (kLifted) m[i] = from[i];
       }
       if (S::kKeyWarps == 1) {
 #pragma unroll
