@@ -12,10 +12,12 @@
 // Two kinds of work:
 //   own     the positions behind the prefix: a unit is (sequence, kv head, up to 64 of its T * group rows), its tiles are 64
 //           of the sequence's own positions. Bound by the bytes of the cache: every key and value is read once, by one CTA
-//           (attend_stream; attend_tiles for block sizes that a TMA box does not fit, about 0.65 of its rate);
+//           (attend_stream; attend_tiles for block sizes that a TMA box does not fit, 0.6 of its rate: 48 ragged sequences
+//           422 us in pages of 24, 254 us in pages of 16);
 //   shared  the prefix's positions: a unit is (kv head, rows of ALL sequences), so each key and value of the prefix is
 //           read once for many rows, not once for every sequence (attend_prefix on tcgen05; attend_tiles for heads of
-//           more than 128 columns and those block sizes). Sequences that end before the prefix does take no part: all their
+//           more than 128 columns and those block sizes: 64 behind 4096 tokens 42 us, 83 us with 256 columns and half the heads,
+//           105 us in pages of 24). Sequences that end before the prefix does take no part: all their
 //           positions are own ones.
 // The tiles of all units are laid end to end and cut into runs, one for each CTA (the own lengths are only known on the
 // device: every CTA adds them up itself). So unequal lengths and few sequences fill the GPU alike. A run's part of a unit is
@@ -45,7 +47,8 @@ constexpr int kPrefixShare = 7;
 constexpr int kPrefixRun = 4;
 // What the shared work's CTAs are expected to take: 9 us and 1.9 us a tile (half where its groups share the tiles). The own
 // work's CTAs that start beside them get so many more tiles, of 2 us, than those that come after (64 behind 4096: 42 us, without
-// 50 us; tiles of 1.5 or 2.6 us 44 us). These only balance the load.
+// 50 us; tiles of 1.5 or 2.6 us 44 us). All of these were set at 128 columns with up to 16 rows a key head and are used for every
+// other shape as they are: they only balance the load, no result depends on them (64 behind 4096 at 64 columns 31 us).
 constexpr int kPrefixCtaNs = 9000, kPrefixTileNs = 1900, kOwnTileNs = 2000;
 constexpr int kMaxBatch = 4096;  // lengths and tile counts of all sequences stay in shared memory
 constexpr float kLog2e = 1.4426950408889634f;

@@ -13,6 +13,8 @@
 // A step is half a tile, 64 positions, so that each group has two S buffers: while it works on one, the tensor cores fill
 // the other. (With one buffer of 128 positions a group waited 1.6 us for its next scores after 1.0 us of work on them: P,
 // which lies over S, had to be used up first.)
+// Two softmax groups that take turns on the tensor cores, and an O that is scaled down only when it has to be, are published
+// techniques (Shah et al. 2024, arXiv 2407.08608; the second T. Dao, Hot Chips 2025).
 // The two groups have a row tile of 128 each of a 256-row unit, or every other tile of positions of a 128-row unit (then
 // they are two pieces). O stays in TMEM. It is scaled down only when a row's maximum has risen by more than 8 (powers of
 // 2) over the one in use; until then weights may reach 2^8, which fp32 sums and 16-bit weights hold as well as 1. (fp16

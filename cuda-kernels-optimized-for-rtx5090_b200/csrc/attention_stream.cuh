@@ -4,7 +4,7 @@
 // attend_tiles from their rate was instructions: 128 threads spent two thirds of them on addresses and copies of 16 bytes,
 // and a block barrier per tile held the warps in step (48 sequences of up to 16001 tokens: 389 us, 4.1 TB/s). Here one
 // warp looks the pages up and issues a TMA box for each page and 64 columns, and the four others only multiply; each
-// goes on as soon as a tile has arrived (mbarriers), whatever the others do: 252 us, 6.3 TB/s or 0.97 of the measured copy
+// goes on as soon as a tile has arrived (mbarriers), whatever the others do: 254 us, 6.2 TB/s or 0.96 of the measured copy
 // bandwidth. With short sequences the 2.5 us before a CTA's first tile, the 0.7 us at the end of each piece and half-filled
 // last tiles show (256 sequences of 256 tokens on average: 4.3 TB/s).
 //

@@ -13,7 +13,8 @@
 // is a G-wide shuffle and nothing goes through shared memory. A group takes up to kNormGroup heads of ONE kind (query, key
 // or value) of a token, so it has one weight, and w cos and w sin are multiplied once for all its heads; the loads of
 // kNormHeads heads are in flight all along, each replaced as soon as its head is worked on. Arithmetic is in pairs (packed
-// fp32). 8 x 4096 tokens of 32 + 8 heads x 128 in bf16 take 129 us, 5.3 TB/s or 0.82 of the measured copy bandwidth. (Groups
+// fp32). 8 x 4096 tokens of 32 + 8 heads x 128 in bf16 take 128 us, 5.3 TB/s or 0.82 of the measured copy bandwidth (with theta
+// 134 us, with the cache write 173 us). (Groups
 // of mixed kinds with the weight and the angles apart took 167 us; lanes that left early, which makes every shuffle of the
 // others ask who is there, 162 us.)
 #pragma once
@@ -61,8 +62,8 @@ __device__ __forceinline__ long long cache_slot(const NormArgs& a, unsigned toke
   return slot < a.cache_slots ? slot : -1;
 }
 
-// Measured at 8 x 4096 tokens of 32 + 8 heads x 128 in bf16: 4 heads in flight of groups of 8 on two CTAs an SM (104 registers)
-// 129 us; 2 heads 140 us; 5 to 8 heads 148 us and more; groups of 4 153 us, of 16 133 us; three CTAs, which spill, 190 us.
+// Measured at 8 x 4096 tokens of 32 + 8 heads x 128 in bf16: 4 heads in flight of groups of 8 on two CTAs an SM (128 registers,
+// 24 bytes of them spilled but for fp16 with theta) 128 us; 2 heads 140 us; 5 to 8 heads 148 us and more; groups of 4 153 us, of 16 133 us; three CTAs, which spill, 190 us.
 constexpr int kNormHeads = 4;  // heads of a group whose loads are in flight
 constexpr int kNormGroup = 8;  // heads of a group at most
 
