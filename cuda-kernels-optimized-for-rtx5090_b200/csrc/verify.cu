@@ -64,10 +64,11 @@ __device__ __forceinline__ void store_remote(double* p, unsigned rank, double v)
 
 // A probability that is NaN or negative counts as 0 (fmaxf drops a NaN), the target's and the draft's alike.
 __device__ __forceinline__ float clean(float p) { return fmaxf(p, 0.0f); }
-// What one element weighs: max(p - q, 0) of the cleaned p and q. A p that is NaN, negative or not above q is taken as q.
+// What one element weighs: max(p - q, 0), of the cleaned p and q: a NaN or negative p is above no cleaned q, and nothing is above
+// an infinite one.
 __device__ __forceinline__ double weight(float p, float q) {
   const float less = clean(q);
-  return (double)fmaxf(p, less) - (double)less;
+  return p > less ? (double)p - (double)less : 0.0;
 }
 
 // A lane's columns of one step, as they were loaded (widened only where they are used, so that several steps' loads fit

@@ -167,3 +167,15 @@ def test_draft_probabilities_that_are_nan_or_negative_count_as_zero(v, dtype):
     q[:, :, ::3] = float("nan")
     q[:, :, 1::3] *= -1.0
     check(p, t, u, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [40, 41, 4096])
+def test_an_infinite_draft_probability_takes_its_column_alone(v, dtype):
+    """max(p - inf, 0) is 0, and the other columns keep theirs: w = (0, 0.125, 0.375) of 0.5."""
+    target, draft = torch.zeros(4, 2, v, dtype=dtype), torch.zeros(4, 1, v, dtype=dtype)
+    target[:, :, 4], target[:, :, 9], target[:, :, v - 1] = 0.25, 0.25, 0.5
+    draft[:, 0, 4], draft[:, 0, 9], draft[:, 0, v - 1] = float("inf"), 0.125, 0.125
+    u = torch.tensor([[0.5, 0.0], [0.5, 0.2], [0.5, 0.3], [0.5, 0.9]])
+    got = check(target, torch.full((4, 1), 4), u, draft)
+    assert got[0][:, 0].tolist() == [9, 9, v - 1, v - 1]
