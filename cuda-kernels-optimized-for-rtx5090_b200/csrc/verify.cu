@@ -15,10 +15,9 @@
 // the CTAs exchange their sums through distributed shared memory, and the one CTA whose slice holds the border reads
 // one warp's part of it again (some KB, from L2), then a sixteenth of that, down to one step of a warp. So there is no
 // workspace, one launch, and a fixed order of additions.
-// 256 sequences of 151936 fp32 columns, each with a refused token (311 MB), take 58.6 us, 5.3 TB/s or 0.82 of the measured copy
-// bandwidth, 1.3 us of it for cleaning the draft's probabilities; 64 of 128256 bf16 columns (31 MB) 13.8 us; one sequence 8.4
-// us, the latency of its chain (token, its probabilities, the row, the exchange, the narrowing). More CTAs than fit at once
-// took 61 to 82 us, three CTAs an SM, which spill, 67 us and more.
+// 256 sequences of 151936 fp32 columns, each with a refused token (311 MB), take 57.5 us, 5.4 TB/s or 0.84 of the measured copy
+// bandwidth; 64 of 128256 bf16 columns (31 MB) 13.9 us; one sequence 8.6 us, the latency of its chain (token,
+// its probabilities, the row, the exchange, the narrowing). More CTAs than fit at once took 61 to 82 us, three CTAs an SM, which spill, 67 us and more.
 #include "ckb200_verify.h"
 #include "common.cuh"
 
@@ -64,28 +63,44 @@ __device__ __forceinline__ void store_remote(double* p, unsigned rank, double v)
 
 // A probability that is NaN or negative counts as 0 (fmaxf drops a NaN), the target's and the draft's alike.
 __device__ __forceinline__ float clean(float p) { return fmaxf(p, 0.0f); }
-// What one element weighs: max(p - q, 0), of the cleaned p and q: a NaN or negative p is above no cleaned q, and nothing is above
-// an infinite one.
-__device__ __forceinline__ double weight(float p, float q) {
-  const float less = clean(q);
-  return p > less ? (double)p - (double)less : 0.0;
-}
+// What one element weighs: max(p - q, 0), q cleaned: a NaN or negative p is above no such q, and nothing is above an infinite one.
+__device__ __forceinline__ double weight(float p, float q) { return p > q ? (double)p - (double)q : 0.0; }
 
 // A lane's columns of one step, as they were loaded (widened only where they are used, so that several steps' loads fit
 // the registers). kVec: one 16-byte vector, else one element. Columns from `end` on are zeros and weigh nothing.
 template <typename T, bool kVec>
 struct Piece {
   static constexpr int N = VecN<T>::N;
+  static constexpr bool kCleanOnce = sizeof(T) == 4;  // by clean_all, not element by element
   uint4 r;
   __device__ __forceinline__ void load(const T* row, int i, int end) {
     r = make_uint4(0u, 0u, 0u, 0u);
     if (row != nullptr && i < end) r = ld_stream(row + i);
   }
   __device__ __forceinline__ void widen(float (&f)[N]) const { unpack16(r, f, (const T*)nullptr); }
+  // Cleans K vectors of fp32. As unsigned integers, negative values and NaN are above infinity, which three-way maxima find with
+  // half an instruction an element; as a rule there are none, and nothing more is done (256 sequences of
+  // 151936 columns 57.5 us; with every element cleaned 59.1 us, with none 57.2 us).
+  template <int K>
+  static __device__ __forceinline__ void clean_all(Piece (&p)[K]) {
+    unsigned most = 0u;
+#pragma unroll
+    for (int s = 0; s < K; ++s) most = __vimax3_u32(__vimax3_u32(most, p[s].r.x, p[s].r.y), p[s].r.z, p[s].r.w);
+    if (most <= 0x7f800000u) return;
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+      float f[N];
+      p[s].widen(f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = clean(f[e]);
+      p[s].r = pack16(f, (const T*)nullptr);
+    }
+  }
 };
 template <typename T>
 struct Piece<T, false> {
   static constexpr int N = 1;
+  static constexpr bool kCleanOnce = false;
   T v;
   __device__ __forceinline__ void load(const T* row, int i, int end) {
     v = row != nullptr && i < end ? row[i] : from_f32<T>(0.0f);
@@ -100,13 +115,13 @@ struct Weights {
   static constexpr int N = Part::N;
   const T *p, *q;
   int without;  // a column that weighs nothing, or -1
-  // The weights of columns i .. i + N - 1.
+  // The weights of columns i .. i + N - 1 (pq cleaned where that is done at once).
   __device__ __forceinline__ void of(const Part& pp, const Part& pq, int i, double (&w)[N]) const {
     float fp[N], fq[N];
     pp.widen(fp);
     pq.widen(fq);
 #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = weight(fp[e], fq[e]);
+    for (int e = 0; e < N; ++e) w[e] = weight(fp[e], Part::kCleanOnce ? fq[e] : clean(fq[e]));
     if ((unsigned)(without - i) < (unsigned)N) {  // asked once for all N columns
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -132,6 +147,7 @@ __device__ __forceinline__ void sum_parts(const Weights<T, kVec>& w, int lo, int
       pp[s].load(w.p, i + s * kStep + lane * N, end);
       pq[s].load(w.q, i + s * kStep + lane * N, end);
     }
+    if constexpr (Piece<T, kVec>::kCleanOnce) Piece<T, kVec>::clean_all(pq);
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
       double some[N];
@@ -256,11 +272,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_rows(const VerifyArgs
     sum_parts(w, lo, hi, sub, warp_sums);
   }
   if (warp != 0) return;
-  Piece<T, kVec> pp, pq;
+  Piece<T, kVec> pp, pq[1];
   pp.load(w.p, lo + lane * N, hi);
-  pq.load(w.q, lo + lane * N, hi);
+  pq[0].load(w.q, lo + lane * N, hi);
+  if constexpr (Piece<T, kVec>::kCleanOnce) Piece<T, kVec>::clean_all(pq);
   double mine[N], sum = 0.0;
-  w.of(pp, pq, lo + lane * N, mine);
+  w.of(pp, pq[0], lo + lane * N, mine);
   int last = -1;  // this lane's last column with any weight
 #pragma unroll
   for (int e = 0; e < N; ++e) {
